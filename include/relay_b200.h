@@ -381,6 +381,34 @@ int rb200_decode_attention_static(const rb200_attn_shape* s, const float* q, con
                                   const int32_t* decode_tokens, int n_decode, int max_ctx, const void* k_pool,
                                   const void* v_pool, void* out, void* stream);
 
+/* No counterpart in the reference. Decode attention for sequences whose contexts begin with the
+ * same keys (samples of one prompt, questions about one document): entries group_off[g] ..
+ * group_off[g + 1] - 1 of decode_tokens are a group whose first prefix_len[g] keys are the same,
+ * so these are read once for the group, through the block table of its first entry, and each
+ * entry's other keys through its own table. The result is that of rb200_decode_attention on
+ * the same batch, up to rounding. q, m, decode_tokens, the pools and out are as there; group_off
+ * (n_groups + 1 entries, ascending) and prefix_len (n_groups) are device arrays.
+ *  - A group counts min(prefix_len[g], context of its first entry) keys as shared; 0 is allowed,
+ *    and so is any length, also one that ends inside a block (the blocks up to there have to hold
+ *    the same keys, they need not be the same blocks). An entry with a shorter context than its
+ *    group's prefix sees its own context only.
+ *  - An entry of decode_tokens below 0, and every entry before group_off[0] or from
+ *    group_off[n_groups] on, is padding: its row of out is left as it was. An entry without keys
+ *    (pos < 0) gets zeros.
+ *  - max_prefix and max_suffix (the longest shared part, the most keys behind it) only decide how
+ *    the work is split over the GPU; other lengths on the device give the same results up to
+ *    rounding. max_prefix 0: nothing is read as shared.
+ *  - scratch (rb200_shared_prefix_scratch_bytes, 16-byte aligned, no initial state) holds the
+ *    shared part's partial results of this call: calls that may overlap need one each.
+ * head_dim 16, 32, 64 or 128, at most 16 query heads per KV head; q 16-byte aligned with
+ * q_stride a multiple of 4, the pools and out 16-byte aligned with o_stride a multiple of 8. */
+size_t rb200_shared_prefix_scratch_bytes(const rb200_attn_shape* s, int n_decode, int n_groups, int max_prefix);
+int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, const rb200_token_meta* m,
+                                  const int32_t* decode_tokens, int n_decode, const int32_t* group_off,
+                                  const int32_t* prefix_len, int n_groups, int max_prefix, int max_suffix,
+                                  const void* k_pool, const void* v_pool, void* scratch, size_t scratch_bytes,
+                                  void* out, void* stream);
+
 /* Causal flash attention for chunks of several tokens over the paged cache (replaces
  * flash_prefill_kernel, engine/src/cuda_kernels.cuh:51-178). tiles[i] = {first batch row,
  * row count <= RB200_PREFILL_ROWS} as built by engine/src/cuda_backend.cu:533-545. */
@@ -435,6 +463,20 @@ int rb200_embed(const int32_t* tokens, const void* table, float* x, int T, int H
 int rb200_qkv_post(float* qkv, const float* bias, const float* inv_freq, const rb200_token_meta* m, int T,
                    void* k_pool, void* v_pool, int heads, int kv_heads, int head_dim, int block_size,
                    void* stream);
+/* No counterpart in the reference. rb200_qkv_post for models that normalise each query and key
+ * head before the rotation: bias, then y = x * rsqrt(mean(x^2) + eps) * weight over each head's
+ * head_dim values (q_norm, k_norm: [head_dim], NULL: no norm), then RoPE on the head's first
+ * rot_dim values (pairs (i, i + rot_dim / 2), the others pass; inv_freq: [rot_dim / 2]), q to q_out
+ * and k and v as fp16 to the token's slot of the paged pools. The angle pos * inv_freq is taken in
+ * 64 bits, so it stays exact at far positions. qkv rows are qkv_stride floats apart, rows of q_out
+ * q_stride; q_out may be qkv itself with the same stride (q in place), any other overlap is
+ * not allowed. Of qkv only that q part is written. A token with seq < 0 or pos < 0 is padding:
+ * nothing of it is read or written. Two tokens of one call must not share a slot. head_dim even and at
+ * most 256; rot_dim even, 0 (inv_freq may be NULL) to head_dim. bias may be NULL. */
+int rb200_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, const float* q_norm, const float* k_norm,
+                        float eps, const float* inv_freq, int rot_dim, const rb200_token_meta* m, int T, float* q_out,
+                        int q_stride, void* k_pool, void* v_pool, int heads, int kv_heads, int head_dim,
+                        int block_size, void* stream);
 /* silu_mul_kernel (engine/src/cuda_backend.cu:245-253): act = silu(g) * u, fp32 [T][2I] -> fp16 [T][ld_act]. */
 int rb200_silu_mul(const float* gu, void* act, int T, int I, int ld_act, void* stream);
 /* f32_to_f16_kernel (engine/src/cuda_backend.cu:110-116): round to nearest even. */
@@ -447,6 +489,33 @@ int rb200_kv_scatter(void* k_pool, void* v_pool, const int32_t* blocks, int n, s
                      const void* staging, void* stream);
 /* Greedy token of each row of logits [R][V] (lowest id wins ties, engine/src/sampler.cpp:17-22). */
 int rb200_argmax_rows(const float* logits, int R, int V, int32_t* token_out, float* logit_out, void* stream);
+/* No counterpart in the reference. What a request asks of its logits ahead of the sampler, row by
+ * row, in this order (each part optional: NULL, or a leading dimension of 0, leaves it out):
+ *  1. penalties: with the row's first history_len tokens of `history` ([R][ld_history]; the first
+ *     prompt_len[r] of them are the prompt, all of them if it is larger, the others were generated),
+ *     a token that occurs in it: x > 0 ? x / repetition : x * repetition; one generated count > 0
+ *     times: x - (frequency * count + presence). `penalties` is a device array of R entries;
+ *     prompt_len NULL: no prompt.
+ *  2. bias_values[r][i] is added to token bias_ids[r][i], i < bias_len[r] ([R][ld_bias]); of
+ *     several entries for one token the last one counts.
+ *  3. mask ([R][ld_mask] words): bit v % 32 of word v / 32 is 0: token v becomes -infinity,
+ *     whatever it was. A row whose mask leaves nothing is -infinity throughout;
+ *     rb200_argmax_rows, and rb200_sample_rows without top-k or nucleus, then answer token 0.
+ * Ids outside [0, V) (padding) are passed over, as are bits behind V; a length above its leading
+ * dimension counts as that, one below 0 as 0. logits and out rows are ld_logits and ld_out
+ * floats apart; out may be logits itself with the same stride, any other overlap is not allowed.
+ * Columns from V on are left as they were. */
+typedef struct rb200_penalties {
+  float repetition; /* > 0; 1: none */
+  float presence;   /* 0: none */
+  float frequency;  /* 0: none */
+  float reserved;   /* 0 */
+} rb200_penalties;
+int rb200_adjust_logits(const float* logits, int ld_logits, float* out, int ld_out, int R, int V,
+                        const rb200_penalties* penalties, const int32_t* history, int ld_history,
+                        const int32_t* history_len, const int32_t* prompt_len, const int32_t* bias_ids,
+                        const float* bias_values, int ld_bias, const int32_t* bias_len, const uint32_t* mask,
+                        int ld_mask, void* stream);
 /* The device sampler on rows of logits [R][V] (engine/src/sampler.cpp:33-105): `params` is a
  * DEVICE array of R entries (see rb200_forward_sample); logprob_out (float64 [R]) may be NULL. */
 int rb200_sample_rows(const float* logits, int R, int V, const rb200_sampling_params* params, int32_t* token_out,

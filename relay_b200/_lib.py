@@ -96,6 +96,9 @@ SIGNATURES = {
     "rb200_decode_plan": (SZ, [C.POINTER(CAttnShape), I, I, P, P]),
     "rb200_decode_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, I, P, P, P, SZ, P, P]),
     "rb200_decode_attention_static": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, I, P, P, P, P]),
+    "rb200_shared_prefix_scratch_bytes": (SZ, [C.POINTER(CAttnShape), I, I, I]),
+    "rb200_shared_prefix_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, P, P, I, I, I, P, P, P, SZ, P,
+                                          P]),
     "rb200_prefill_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, P, P, P, P]),
     "rb200_reference_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), I, P, P, P, P]),
     "rb200_gemv_scratch_bytes": (SZ, [I, I]),
@@ -106,11 +109,13 @@ SIGNATURES = {
     "rb200_rmsnorm": (I, [P, P, P, P, I, I, I, F, P]),
     "rb200_embed": (I, [P, P, P, I, I, I, P]),
     "rb200_qkv_post": (I, [P, P, P, C.POINTER(CTokenMeta), I, P, P, I, I, I, I, P]),
+    "rb200_qkv_norm_post": (I, [P, I, P, P, P, F, P, I, C.POINTER(CTokenMeta), I, P, I, P, P, I, I, I, I, P]),
     "rb200_silu_mul": (I, [P, P, I, I, I, P]),
     "rb200_f32_to_f16": (I, [P, P, SZ, P]),
     "rb200_kv_gather": (I, [P, P, P, I, SZ, P, P]),
     "rb200_kv_scatter": (I, [P, P, P, I, SZ, P, P]),
     "rb200_argmax_rows": (I, [P, I, I, P, P, P]),
+    "rb200_adjust_logits": (I, [P, I, P, I, I, I, P, P, I, P, P, P, P, I, P, P, I, P]),
     "rb200_sample_rows": (I, [P, I, I, P, P, P, P]),
 }
 

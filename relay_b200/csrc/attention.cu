@@ -22,6 +22,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "attn_tiles.cuh"
 #include "kernels.h"
 #include "tcgen05.cuh"
 
@@ -31,65 +32,9 @@ namespace {
 
 constexpr int kDecWarps = 4;    // independent tile workers per decode CTA
 constexpr int kDecStages = 3;   // 16-key tiles in flight per warp
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Halves from the start of one layer's pool to row `key` of KV head `kvh`.
-// `table` is indexed by absolute block number of the sequence minus `first_block`.
-__device__ __forceinline__ long long key_offset(const int* table, int first_block, int key, int bs, int bs_shift,
-                                                int kv_heads, int kvh, int D) {
-  int blk_i, slot;
-  if (bs_shift >= 0) {
-    blk_i = key >> bs_shift;
-    slot = key & (bs - 1);
-  } else {
-    blk_i = key / bs;
-    slot = key - blk_i * bs;
-  }
-  const long long blk = table[blk_i - first_block];
-  return ((blk * kv_heads + kvh) * bs + slot) * static_cast<long long>(D);
-}
-
 // ---------------------------------------------------------------------------------------
 // Split-context decode
 // ---------------------------------------------------------------------------------------
-
-// Shared by decode and prefill: scores of 16 query rows against 16 keys.
-// s[0] covers keys 0-7 of the tile, s[1] keys 8-15; ktile is [16][D] halves, swizzled.
-template <int D>
-__device__ __forceinline__ void qk_16x16(float (&s)[2][4], const uint32_t (&qf)[D / 16][4], uint32_t ktile, int lane) {
-  constexpr int CH = D / 8;
-  const int row = (lane & 7) + ((lane >> 4) << 3);
-  const int csel = (lane >> 3) & 1;
-#pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) {
-    uint32_t kb[4];
-    ldmatrix_x4(kb, ktile + swz<CH>(row, 2 * kk + csel) * 16);
-    mma_f16(s[0], qf[kk], kb[0], kb[1]);
-    mma_f16(s[1], qf[kk], kb[2], kb[3]);
-  }
-}
-
-// O(16 x D) += P(16 x 16 keys) V(16 keys x D); vtile is [16][D] halves, swizzled.
-template <int D>
-__device__ __forceinline__ void pv_16x16(float (&o)[D / 8][4], const uint32_t (&pa)[4], uint32_t vtile, int lane) {
-  constexpr int CH = D / 8;
-  const int row = (lane & 7) + (((lane >> 3) & 1) << 3);
-  const int csel = lane >> 4;
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
-    uint32_t vb[4];
-    ldmatrix_x4_trans(vb, vtile + swz<CH>(row, 2 * j + csel) * 16);
-    mma_f16(o[2 * j], pa, vb[0], vb[1]);
-    mma_f16(o[2 * j + 1], pa, vb[2], vb[3]);
-  }
-}
 
 template <int D>
 constexpr size_t decode_smem_bytes() {
@@ -645,13 +590,6 @@ reference_attention_kernel(const float* __restrict__ q, TokenMeta m, const __hal
   __half* o = out + static_cast<long long>(t) * o_stride + h * D;
   if (threadIdx.x < D) o[threadIdx.x] = __float2half_rn(acc0 / run_l);
   if (threadIdx.x + 128 < D) o[threadIdx.x + 128] = __float2half_rn(acc1 / run_l);
-}
-
-int shift_of(int bs) {
-  if (bs <= 0 || (bs & (bs - 1)) != 0) return -1;
-  int s = 0;
-  while ((1 << s) < bs) ++s;
-  return s;
 }
 
 template <class K>

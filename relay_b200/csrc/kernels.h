@@ -88,6 +88,23 @@ void launch_prefill_attention(const AttnShape& s, const float* q, const TokenMet
 void launch_reference_attention(const AttnShape& s, const float* q, const TokenMeta& m, int T, const __half* kc,
                                 const __half* vc, __half* out, cudaStream_t st);
 
+// ---- qkv_norm.cu ----
+void launch_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, const float* q_norm, const float* k_norm, float eps,
+                          const float* inv_freq, int rot, const TokenMeta& m, int T, float* q_out, int q_stride, __half* kc,
+                          __half* vc, int heads, int kv_heads, int D, int block_size, cudaStream_t st);
+
+// ---- shared_prefix.cu ----
+size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix);
+void launch_shared_prefix_attention(const AttnShape& s, const float* q, const TokenMeta& m, const int* decode_tokens, int n_decode,
+                                    const int* group_off, const int* prefix_len, int n_groups, int max_prefix, int max_suffix,
+                                    const __half* kc, const __half* vc, float* scratch, __half* out, cudaStream_t st);
+
+// ---- logits.cu ----
+void launch_adjust_logits(const float* logits, int ld_logits, float* out, int ld_out, int R, int V, const rb200_penalties* penalties,
+                          const int* history, int ld_history, const int* history_len, const int* prompt_len, const int* bias_ids,
+                          const float* bias_values, int ld_bias, const int* bias_len, const uint32_t* mask, int ld_mask,
+                          cudaStream_t st);
+
 // ---- gemm.cu ----
 // A weight matrix [N][ld] in device memory: fp16, or int8 with one fp32 scale per row.
 // ld >= K is the row stride in elements; columns K..ld-1 hold zeros.
