@@ -15,6 +15,15 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// (x, y) as two pairs of halves, x = hi + lo to 2^-22 of x (2^-25 where lo is subnormal). With hi alone
+// the rounding of q would cost an attention output about as much as its own rounding to fp16.
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 b = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = pack_half2(x - b.x, y - b.y);
+}
+
 // Halves from the start of one layer's pool to row `key` of KV head `kvh`.
 // `table` is indexed by absolute block number of the sequence minus `first_block`.
 __device__ __forceinline__ long long key_offset(const int* table, int first_block, int key, int bs, int bs_shift,

@@ -8,98 +8,22 @@
 // product of matrices: (tokens x heads of a KV head) rows against P keys, each key read once per row
 // tile instead of once per token. Two kernels:
 //
-//  * prefix_mma_kernel: a CTA takes 64 rows (token, head) of one group and KV head and a slice
-//    of the shared keys, and leaves a partial (m, l, o) per row;
+//  * umma_prefix_kernel (umma_prefix.cu; head sizes 64 and 128, block sizes that are multiples of 16) or
+//    prefix_mma_kernel (the other layouts): a CTA takes 128 or 64 rows (token, head) of one group and
+//    KV head and a slice of the shared keys, and leaves a partial (m, l, o) per row;
 //  * suffix_kernel: a CTA takes one token and KV head (or a slice of its own keys, the slices
 //    as one cluster), streams the keys behind the prefix, adds the partials of the prefix and writes
-//    the output.
+//    the output. It starts under the tail of the first kernel and waits for it only ahead of the join.
+//
+// Scores take q in full (two fp16 halves, split_half2); the weights round to fp16 for the second product.
 #include "attn_tiles.cuh"
 #include "kernels.h"
+#include "prefix_groups.cuh"
 #include "tcgen05.cuh"
 
 namespace rb200 {
 
 namespace {
-
-constexpr int kSlice = 128;  // slices of the shared keys are multiples of this
-
-// The group geometry on the device.
-struct Groups {
-  const int* decode_tokens;
-  const int* off;         // [n_groups + 1]
-  const int* prefix_len;  // [n_groups]; null: nothing is shared
-  int n_decode, n_groups;
-};
-
-// Partial results of the shared part: o [n_decode * heads][parts][D], then (max in log2 units, sum)
-// [n_decode * heads][parts]. Slice p of a prefix of P keys starts at p * slice_of(P, parts); slices
-// that start at or behind P are neither written nor read.
-struct Partials {
-  float* o;
-  float* ml;
-  int parts;
-};
-
-__device__ __forceinline__ int slice_of(int P, int parts) { return (((P + parts - 1) / parts) + kSlice - 1) / kSlice * kSlice; }
-
-// How many keys the group [lo, hi) shares, and the block table that names them.
-struct Prefix {
-  int keys;
-  const int* table;
-};
-__device__ __forceinline__ Prefix prefix_of(const Groups& gr, const TokenMeta& m, int g, int lo, int hi) {
-  int tok = -1;
-  for (int i = lo; i < hi && tok < 0; ++i) tok = gr.decode_tokens[i];  // the first entry that is not padding
-  if (tok < 0 || gr.prefix_len == nullptr) return {0, nullptr};
-  const int keys = min(gr.prefix_len[g], m.pos[tok] + 1);
-  if (keys <= 0) return {0, nullptr};
-  return {keys, m.tables + m.table_off[m.seq[tok]]};
-}
-
-// Entries [lo, hi) of group g; bounds that do not fit the batch are cut to it.
-__device__ __forceinline__ void group_bounds(const Groups& gr, int g, int& lo, int& hi) {
-  lo = max(gr.off[g], 0);
-  hi = min(gr.off[g + 1], gr.n_decode);
-}
-
-// The x-th row tile over all groups, a group of n entries having ceil(n * G / rows) of them. Called by
-// whole warps; every lane gets the answer. False behind the last tile.
-__device__ __forceinline__ bool find_tile(const Groups& gr, int G, int rows, int x, int& g, int& tile) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int g0 = 0; g0 < gr.n_groups; g0 += 32) {
-    int n = 0;
-    if (g0 + lane < gr.n_groups) {
-      int lo, hi;
-      group_bounds(gr, g0 + lane, lo, hi);
-      n = (max(hi - lo, 0) * G + rows - 1) / rows;
-    }
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, before + incl > x);
-    if (past) {
-      const int src = __ffs(past) - 1;
-      g = g0 + src;
-      tile = x - before - __shfl_sync(0xffffffffu, incl - n, src);
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return false;
-}
-
-// The group that entry di belongs to, or -1.
-__device__ __forceinline__ int group_of(const Groups& gr, int di) {
-  const int lane = threadIdx.x & 31;
-  int n = 0;  // offsets at or before di
-  for (int j0 = 0; j0 <= gr.n_groups; j0 += 32)
-    n += __popc(__ballot_sync(0xffffffffu, j0 + lane <= gr.n_groups && gr.off[min(j0 + lane, gr.n_groups)] <= di));
-  return n >= 1 && n <= gr.n_groups ? n - 1 : -1;
-}
 
 // ---------------------------------------------------------------------------------------
 // The shared keys
@@ -121,8 +45,8 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
   constexpr int STAGE_HALVES = 2 * kPxKeys * D;  // K tile then V tile
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const uint32_t smem0 = smem_u32(smem_raw);
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // behind the wait: what suffix_kernel reads early is then complete
   const int G = heads / kv_heads, kvh = blockIdx.y;
   int g = 0, tile = 0, lo, hi;
   if (!find_tile(gr, G, kPxRows, blockIdx.x, g, tile)) return;
@@ -147,7 +71,7 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
     if (tok < 0) entry[r] = -1;
     qrow[r] = q + static_cast<long long>(max(tok, 0)) * q_stride + head[r] * D;
   }
-  uint32_t qf[D / 16][4];
+  uint32_t qf[D / 16][4], ql[D / 16][4];
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     const int d0 = kk * 16 + 2 * t4;
@@ -158,10 +82,8 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
         v[r][0] = *reinterpret_cast<const float2*>(qrow[r] + d0);
         v[r][1] = *reinterpret_cast<const float2*>(qrow[r] + d0 + 8);
       }
-    qf[kk][0] = pack_half2(v[0][0].x, v[0][0].y);
-    qf[kk][1] = pack_half2(v[1][0].x, v[1][0].y);
-    qf[kk][2] = pack_half2(v[0][1].x, v[0][1].y);
-    qf[kk][3] = pack_half2(v[1][1].x, v[1][1].y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split_half2(v[e & 1][e >> 1].x, v[e & 1][e >> 1].y, qf[kk][e], ql[kk][e]);
   }
 
   auto load_stage = [&](int kt, int stage) {
@@ -200,6 +122,7 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
     for (int kp = 0; kp < kPxKeys / 16; ++kp) {
       float s2[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       qk_16x16<D>(s2, qf, ktile + kp * 16 * D * 2, lane);
+      qk_16x16<D>(s2, ql, ktile + kp * 16 * D * 2, lane);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[2 * kp][e] = s2[0][e];
@@ -292,7 +215,7 @@ template <int D, bool CONTIG, bool WIDE>
 __global__ void __launch_bounds__(kSxWarps * 32, 2)
 suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half* __restrict__ kc, const __half* __restrict__ vc,
               Partials px, __half* __restrict__ out, int heads, int kv_heads, int bs, int bs_shift, int q_stride, int o_stride,
-              float scale_log2e) {
+              float scale_log2e, int early) {
   constexpr int CH = D / 8;
   constexpr int TILE_HALVES = 16 * D;
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -300,45 +223,51 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   __shared__ float j_m[16], j_l[16];  // this CTA's (max, sum) per head
 
   pdl_trigger();
-  pdl_wait();
+  // `early`: the kernel ahead is a prefix kernel, all of whose CTAs have waited for what came before them, so
+  // the metadata, q and the pages are complete (read from L2); only its partials have to be waited for.
+  if (!early) pdl_wait();
   const int di = blockIdx.x, kvh = blockIdx.y, slices = gridDim.z, rank = blockIdx.z;
-  const int tok = gr.decode_tokens[di];
+  const int tok = __ldcg(gr.decode_tokens + di);
   const int g = group_of(gr, di);
-  if (tok < 0 || g < 0) return;  // padding: the whole cluster leaves
+  if (tok < 0 || g < 0) {  // padding: the whole cluster leaves
+    pdl_wait();
+    return;
+  }
   int lo, hi;
   group_bounds(gr, g, lo, hi);
   const int P = prefix_of(gr, m, g, lo, hi).keys;
-  const int ctx = max(m.pos[tok] + 1, 0), start = min(P, ctx);
+  const int ctx = max(__ldcg(m.pos + tok) + 1, 0), start = min(P, ctx);
   // Tiles start at multiples of 16 where a tile has to be a run of a page; keys before `start` are masked.
   const int base = CONTIG ? start & ~15 : start;
   const int per = ((ctx - base + slices - 1) / slices + 15) & ~15;
   const int k0 = min(base + rank * per, ctx), k1 = min(k0 + per, ctx);
   const int ntiles = (k1 - k0 + 15) >> 4;
-  const int* table = ctx > 0 ? m.tables + m.table_off[m.seq[tok]] : nullptr;
+  const int* table = ctx > 0 ? m.tables + __ldcg(m.table_off + __ldcg(m.seq + tok)) : nullptr;
 
   const int G = heads / kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, t4 = lane & 3;
 
-  uint32_t qf[D / 16][4];
+  // The heads' queries as A fragments: rows 0..7 hi of heads 0..7; rows 8..15 hi of heads 8..15 (then the lo
+  // halves need fragments of their own) or, with up to 8 heads, their lo, so that one product makes both.
+  uint32_t qf[D / 16][4], ql[WIDE ? D / 16 : 1][4];
   {
     const float* q0 = q + static_cast<long long>(tok) * q_stride + (kvh * G) * D;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-      const int d0 = kk * 16 + 2 * t4;
-      float2 a = make_float2(0.f, 0.f), b = a, c = a, e = a;
-      if (gid < G) {
-        a = *reinterpret_cast<const float2*>(q0 + gid * D + d0);
-        c = *reinterpret_cast<const float2*>(q0 + gid * D + d0 + 8);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d0 = kk * 16 + 2 * t4 + 8 * e;
+        float2 a = make_float2(0.f, 0.f), b = a;
+        if (gid < G) a = __ldcg(reinterpret_cast<const float2*>(q0 + gid * D + d0));
+        if constexpr (WIDE) {
+          if (gid + 8 < G) b = __ldcg(reinterpret_cast<const float2*>(q0 + (gid + 8) * D + d0));
+          split_half2(a.x, a.y, qf[kk][2 * e], ql[kk][2 * e]);
+          split_half2(b.x, b.y, qf[kk][2 * e + 1], ql[kk][2 * e + 1]);
+        } else {
+          split_half2(a.x, a.y, qf[kk][2 * e], qf[kk][2 * e + 1]);
+        }
       }
-      if (WIDE && gid + 8 < G) {
-        b = *reinterpret_cast<const float2*>(q0 + (gid + 8) * D + d0);
-        e = *reinterpret_cast<const float2*>(q0 + (gid + 8) * D + d0 + 8);
-      }
-      qf[kk][0] = pack_half2(a.x, a.y);
-      qf[kk][1] = pack_half2(b.x, b.y);
-      qf[kk][2] = pack_half2(c.x, c.y);
-      qf[kk][3] = pack_half2(e.x, e.y);
     }
   }
 
@@ -349,7 +278,7 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   const int my_tiles = ntiles > warp ? (ntiles - warp + kSxWarps - 1) / kSxWarps : 0;
   auto fetch_ids = [&](int j0) {
     const int j = j0 + lane, key = k0 + (warp + j * kSxWarps) * 16;
-    return CONTIG && j < my_tiles ? table[bs_shift >= 0 ? key >> bs_shift : key / bs] : 0;
+    return CONTIG && j < my_tiles ? __ldcg(table + (bs_shift >= 0 ? key >> bs_shift : key / bs)) : 0;
   };
   int ids = fetch_ids(0), ids_next = fetch_ids(32);
   auto load_tile = [&](int j) {
@@ -408,6 +337,15 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
     const uint32_t vtile = ktile + TILE_HALVES * 2;
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     qk_16x16<D>(s, qf, ktile, lane);
+    if constexpr (WIDE) {
+      qk_16x16<D>(s, ql, ktile, lane);
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        s[nt][0] += s[nt][2];
+        s[nt][1] += s[nt][3];
+      }
+    }
 
     const int key0 = k0 + (warp + j * kSxWarps) * 16 + 2 * t4;
     float corr[2];
@@ -464,6 +402,7 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
     *reinterpret_cast<float2*>(os + gid * D + i * 8 + 2 * t4) = make_float2(o[i][0], o[i][1]);
     if constexpr (WIDE) *reinterpret_cast<float2*>(os + (gid + 8) * D + i * 8 + 2 * t4) = make_float2(o[i][2], o[i][3]);
   }
+  if (early) pdl_wait();
   __syncthreads();
 
   const float* os_all = reinterpret_cast<const float*>(smem_raw);
@@ -541,16 +480,34 @@ long long row_tiles(const AttnShape& s, int n_decode, int n_groups, int rows) {
   return (static_cast<long long>(n_decode) * (s.heads / s.kv_heads) + static_cast<long long>(n_groups) * (rows - 1)) / rows;
 }
 
-// Slices of the shared keys: enough CTAs for one wave of the GPU.
-int prefix_parts(long long tiles, int kv_heads, int max_prefix) {
-  const long long ctas = std::max<long long>(1, tiles * kv_heads);
-  const long long most = std::max(1, div_up(max_prefix, 2 * kSlice));
-  return static_cast<int>(std::max<long long>(1, std::min({2LL * sm_count() / ctas, most, 64LL})));
+// Into how many slices the longest prefix is cut: the number that keeps the last SM busy for the shortest
+// time, a CTA costing its keys and as much as kSetupKeys more to start and to leave its partials.
+constexpr int kSetupKeys = 256;
+int prefix_parts(long long ctas, long long slots, int max_prefix) {
+  int best = 1;
+  long long least = -1;
+  for (int p = 1; p <= 64 && (p == 1 || max_prefix > (p - 1) * 2 * kPrefixSlice); ++p) {
+    const long long keys = (div_up(max_prefix, p) + kPrefixSlice - 1LL) / kPrefixSlice * kPrefixSlice;
+    const long long cost = (ctas * p + slots - 1) / slots * (keys + kSetupKeys);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = p;
+    }
+  }
+  return best;
+}
+
+int prefix_rows(const AttnShape& s) { return umma_prefix_usable(s) ? kUmmaPrefixRows : kPxRows; }
+
+// One CTA of the tcgen05 kernel fits an SM, two of the other.
+int parts_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix) {
+  const long long ctas = row_tiles(s, n_decode, n_groups, prefix_rows(s)) * s.kv_heads;
+  return prefix_parts(ctas, (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count(), max_prefix);
 }
 
 template <int D, bool CONTIG, bool WIDE>
 void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const __half* kc, const __half* vc,
-                   const Partials& px, __half* out, int slices, float scale_log2e, cudaStream_t st) {
+                   const Partials& px, __half* out, int slices, float scale_log2e, int early, cudaStream_t st) {
   static PerDeviceOnce once;
   auto kernel = suffix_kernel<D, CONTIG, WIDE>;
   if (once.first())
@@ -571,36 +528,37 @@ void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const
   cfg.numAttrs = slices > 1 ? 2 : 1;
   count_launch();
   const int heads = s.heads, kv_heads = s.kv_heads, bs = s.block_size, shift = shift_of(s.block_size), qs = s.q_stride, os = s.o_stride;
-  RB_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, m, gr, kc, vc, px, out, heads, kv_heads, bs, shift, qs, os, scale_log2e));
+  RB_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, m, gr, kc, vc, px, out, heads, kv_heads, bs, shift, qs, os, scale_log2e, early));
 }
 
 template <int D>
 void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, int max_prefix, int max_suffix,
               const __half* kc, const __half* vc, Partials px, __half* out, cudaStream_t st) {
   const float scale_log2e = kLog2e / sqrtf(static_cast<float>(D));
-  if (max_prefix > 0) {
-    static PerDeviceOnce once;
-    auto kernel = prefix_mma_kernel<D>;
-    if (once.first())
-      RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(prefix_smem_bytes<D>())));
-    const dim3 grid(static_cast<unsigned>(row_tiles(s, gr.n_decode, gr.n_groups, kPxRows)), s.kv_heads, px.parts);
-    count_launch();
-    launch_pdl(kernel, grid, dim3(128), prefix_smem_bytes<D>(), st, q, m, gr, kc, vc, px, s.heads, s.kv_heads, s.block_size,
-               shift_of(s.block_size), s.q_stride, scale_log2e);
+  const int early = max_prefix > 0;
+  if (early) {
+    const long long tiles = row_tiles(s, gr.n_decode, gr.n_groups, prefix_rows(s));
+    if (umma_prefix_usable(s)) {
+      launch_umma_prefix(s, q, m, gr, kc, vc, px, static_cast<int>(tiles), st);
+    } else {
+      static PerDeviceOnce once;
+      auto kernel = prefix_mma_kernel<D>;
+      if (once.first())
+        RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(prefix_smem_bytes<D>())));
+      count_launch();
+      launch_pdl(kernel, dim3(static_cast<unsigned>(tiles), s.kv_heads, px.parts), dim3(128), prefix_smem_bytes<D>(), st, q, m, gr, kc, vc,
+                 px, s.heads, s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, scale_log2e);
+    }
   }
   // A few tokens with many keys of their own: up to eight CTAs of at least 128 keys for each (token, KV head).
   const long long pairs = static_cast<long long>(gr.n_decode) * s.kv_heads;
   int slices = 1;
   while (slices < 8 && pairs * slices * 2 <= 2LL * sm_count() && max_suffix / (slices * 2) >= 128) slices *= 2;
   const bool contig = s.block_size % 16 == 0, wide = s.heads / s.kv_heads > 8;
-  if (contig && !wide) launch_suffix<D, true, false>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, st);
-  else if (contig) launch_suffix<D, true, true>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, st);
-  else if (!wide) launch_suffix<D, false, false>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, st);
-  else launch_suffix<D, false, true>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, st);
-}
-
-int parts_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix) {
-  return prefix_parts(row_tiles(s, n_decode, n_groups, kPxRows), s.kv_heads, max_prefix);
+  if (contig && !wide) launch_suffix<D, true, false>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
+  else if (contig) launch_suffix<D, true, true>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
+  else if (!wide) launch_suffix<D, false, false>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
+  else launch_suffix<D, false, true>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
 }
 
 }  // namespace

@@ -180,6 +180,19 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// Descriptor of an MN-major operand (V: [key][d], d contiguous) in the layout TMA's 128-byte
+// swizzle writes: 8-key groups 1024 bytes apart (stride byte offset), 64-wide d atoms
+// `lbo_bytes` apart (leading byte offset), version 1, layout type SWIZZLE_128B.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr, uint32_t lbo_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFF) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
 // Instruction descriptor for kind::f16: fp32 accumulator (bits 4-5 = 1), fp16 A and B
 // (bits 7-9, 10-12 = 0), both K-major (bits 15, 16 = 0), N / 8 in bits 17-22, M / 16 in bits 24-28.
 __host__ __device__ constexpr uint32_t umma_idesc(int M, int N) {

@@ -54,19 +54,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Descriptor of an MN-major operand (V: [key][d], d contiguous) in the layout TMA's 128-byte
-// swizzle writes: 8-key groups 1024 bytes apart (stride byte offset), 64-wide d atoms
-// `lbo_bytes` apart (leading byte offset), version 1, layout type SWIZZLE_128B.
-__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr, uint32_t lbo_bytes) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
-  d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFF) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-
 template <int D>
 struct PfSmem {
   static constexpr int kQBytes = kRows * D * 2;
