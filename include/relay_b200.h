@@ -471,7 +471,7 @@ int rb200_qkv_post(float* qkv, const float* bias, const float* inv_freq, const r
  * 64 bits, so it stays exact at far positions. qkv rows are qkv_stride floats apart, rows of q_out
  * q_stride; q_out may be qkv itself with the same stride (q in place), any other overlap is
  * not allowed. Of qkv only that q part is written. A token with seq < 0 or pos < 0 is padding:
- * nothing of it is read or written. Two tokens of one call must not share a slot. head_dim even and at
+ * its row of q_out stays as it was and nothing is appended. Two tokens of one call must not share a slot. head_dim even and at
  * most 256; rot_dim even, 0 (inv_freq may be NULL) to head_dim. bias may be NULL. */
 int rb200_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, const float* q_norm, const float* k_norm,
                         float eps, const float* inv_freq, int rot_dim, const rb200_token_meta* m, int T, float* q_out,

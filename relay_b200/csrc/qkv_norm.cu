@@ -5,14 +5,17 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)  on the pairs (i, i + rot/2) of y
 //
 // Every value is read once and written once: 4 (Q + 2 KV) bytes of a token come in, 4 Q + 4 KV go
-// out, so the kernel is bound by memory, and by latency for a few tokens.
+// out, so the kernel is bound by memory, and by latency for a few tokens. Heads whose rows are whole
+// 16-byte vectors take qkv_norm_vec_kernel, which keeps a head in the registers of 8, 16 or 32 lanes;
+// the others (head_dim not a multiple of 4, rot_dim not of 8, unaligned rows) qkv_norm_post_kernel.
 #include "kernels.h"
 
 namespace rb200 {
 
 namespace {
 
-constexpr int kQnWarps = 8;
+constexpr int kQnWarps = 8;   // of qkv_norm_post_kernel
+constexpr int kQnRounds = 4;  // heads of a warp in flight in qkv_norm_vec_kernel
 
 // cos and sin of pos * inv_freq. The product is exact in float64 and reduced there: its float32
 // rounding alone would be off by 4e-3 rad at position 131072. What is left, at most pi, rounds to
@@ -22,6 +25,119 @@ __device__ __forceinline__ void rotation(int pos, float inv_freq, float& c, floa
   const double a = static_cast<double>(pos) * static_cast<double>(inv_freq);
   const double r = fma(-rint(a * (1.0 / kTwoPi)), kTwoPi, a);
   sincosf(static_cast<float>(r), &s, &c);
+}
+
+// One CTA per token. A head is held by LPH lanes, lane l with the vectors (4 values) l and, with NV = 2,
+// l + LPH; a warp takes 32 / LPH heads at a time and has U such rounds in flight, so that a token's
+// whole row is under way before anything waits: with 12 warps 24 KB at 32 + 2 x 8 heads of 128. The
+// rotation angles and the page lookup (three dependent loads) run under those loads. The partner of
+// a rotated vector is rot/8 vectors away, in another lane: it comes by shuffle.
+template <int LPH, int NV>
+__global__ void __launch_bounds__(512)
+qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const float* __restrict__ q_norm,
+                    const float* __restrict__ k_norm, float eps, const float* __restrict__ inv_freq, int rot, TokenMeta m,
+                    float* q_out, __half* __restrict__ kc, __half* __restrict__ vc, int heads, int kv_heads, int D, int bs,
+                    int qkv_stride, int q_stride) {
+  constexpr int HPW = 32 / LPH, U = kQnRounds;
+  extern __shared__ float sm[];  // [rot/2] cos, [rot/2] sin
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x, half = rot >> 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int sub = lane / LPH, l = lane % LPH;
+  const int vecs = D >> 2, h4 = rot >> 3;  // vectors of a head; how far a rotated vector's partner is
+  const int total = heads + 2 * kv_heads;
+  const int seq = m.seq[t], p = m.pos[t];
+  const float* src = qkv + static_cast<long long>(t) * qkv_stride;
+  float* dst = q_out + static_cast<long long>(t) * q_stride;
+  long long block = 0;
+  int slot = 0;
+  float4 wq[NV], wk[NV];
+  for (int h0 = 0; h0 < total; h0 += warps * HPW * U) {
+    float4 x[U][NV];
+    int head[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + (u * warps + warp) * HPW + sub;
+      head[u] = h;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int v = l + n * LPH;
+        x[u][n] = h < total && v < vecs ? *reinterpret_cast<const float4*>(src + h * D + v * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    if (h0 == 0) {
+      if (seq < 0 || p < 0) return;  // padding; looked at only here so that the row's loads do not wait for it
+      for (int i = threadIdx.x; i < half; i += blockDim.x) rotation(p, inv_freq[i], sm[i], sm[half + i]);
+      block = m.tables[m.table_off[seq] + p / bs];
+      slot = p % bs;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int v = l + n * LPH;
+        wq[n] = q_norm && v < vecs ? reinterpret_cast<const float4*>(q_norm)[v] : make_float4(1.f, 1.f, 1.f, 1.f);
+        wk[n] = k_norm && v < vecs ? reinterpret_cast<const float4*>(k_norm)[v] : make_float4(1.f, 1.f, 1.f, 1.f);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = head[u];
+      const bool is_q = h < heads, is_v = h >= heads + kv_heads;
+      float ss = 0.f;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int v = l + n * LPH;
+        if (bias && h < total && v < vecs) {
+          const float4 b = *reinterpret_cast<const float4*>(bias + h * D + v * 4);
+          x[u][n].x += b.x, x[u][n].y += b.y, x[u][n].z += b.z, x[u][n].w += b.w;
+        }
+        ss += x[u][n].x * x[u][n].x + x[u][n].y * x[u][n].y + x[u][n].z * x[u][n].z + x[u][n].w * x[u][n].w;
+      }
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (!is_v && (is_q ? q_norm : k_norm)) {
+        const float scale = 1.0f / sqrtf(ss / static_cast<float>(D) + eps);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const float4 w = is_q ? wq[n] : wk[n];
+          x[u][n].x *= scale * w.x, x[u][n].y *= scale * w.y, x[u][n].z *= scale * w.z, x[u][n].w *= scale * w.w;
+        }
+      }
+      float4 y[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        // vector v of the head and its partner: v + h4 for the first h4 vectors, v - h4 for the next h4
+        const int v = l + n * LPH, pv = v < h4 ? v + h4 : v - h4;
+        const int from = sub * LPH + (pv & (LPH - 1));
+        float4 z;
+        z.x = __shfl_sync(0xffffffffu, x[u][0].x, from), z.y = __shfl_sync(0xffffffffu, x[u][0].y, from);
+        z.z = __shfl_sync(0xffffffffu, x[u][0].z, from), z.w = __shfl_sync(0xffffffffu, x[u][0].w, from);
+        if constexpr (NV == 2) {
+          const float4 z1 = make_float4(__shfl_sync(0xffffffffu, x[u][1].x, from), __shfl_sync(0xffffffffu, x[u][1].y, from),
+                                        __shfl_sync(0xffffffffu, x[u][1].z, from), __shfl_sync(0xffffffffu, x[u][1].w, from));
+          if (pv >= LPH) z = z1;
+        }
+        y[n] = x[u][n];
+        if (!is_v && v < 2 * h4) {
+          const int i = (v < h4 ? v : pv) * 4;
+          const float4 c = *reinterpret_cast<const float4*>(sm + i), sn = *reinterpret_cast<const float4*>(sm + half + i);
+          const float g = v < h4 ? -1.f : 1.f;
+          y[n].x = x[u][n].x * c.x + g * (z.x * sn.x), y[n].y = x[u][n].y * c.y + g * (z.y * sn.y);
+          y[n].z = x[u][n].z * c.z + g * (z.z * sn.z), y[n].w = x[u][n].w * c.w + g * (z.w * sn.w);
+        }
+      }
+      if (h >= total) continue;
+      const int kvh = is_v ? h - heads - kv_heads : h - heads;
+      __half* page = (is_v ? vc : kc) + ((block * kv_heads + kvh) * bs + slot) * D;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int v = l + n * LPH;
+        if (v >= vecs) continue;
+        if (is_q) *reinterpret_cast<float4*>(dst + h * D + v * 4) = y[n];
+        else *reinterpret_cast<uint2*>(page + v * 4) = make_uint2(pack_half2(y[n].x, y[n].y), pack_half2(y[n].z, y[n].w));
+      }
+    }
+  }
 }
 
 // One CTA per token, one warp per head at a time; the head's values pass through the warp's own
@@ -82,6 +198,17 @@ void launch_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, c
                           __half* vc, int heads, int kv_heads, int D, int block_size, cudaStream_t st) {
   if (T == 0) return;
   count_launch();
+  auto aligned = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (D % 4 == 0 && rot % 8 == 0 && qkv_stride % 4 == 0 && q_stride % 4 == 0 && aligned(qkv, 16) && aligned(q_out, 16) &&
+      aligned(bias, 16) && aligned(q_norm, 16) && aligned(k_norm, 16) && aligned(kc, 8) && aligned(vc, 8)) {
+    const int lanes = D > 64 ? 32 : (D > 32 ? 16 : 8);
+    const int warps = std::min(16, std::max(1, div_up(heads + 2 * kv_heads, 32 / lanes * kQnRounds)));
+    auto kernel = D > 128 ? qkv_norm_vec_kernel<32, 2>
+                          : (lanes == 32 ? qkv_norm_vec_kernel<32, 1> : (lanes == 16 ? qkv_norm_vec_kernel<16, 1> : qkv_norm_vec_kernel<8, 1>));
+    launch_pdl(kernel, dim3(T), dim3(warps * 32), rot * sizeof(float), st, qkv, bias, q_norm, k_norm, eps, inv_freq, rot, m, q_out, kc, vc,
+               heads, kv_heads, D, block_size, qkv_stride, q_stride);
+    return;
+  }
   const size_t smem = (static_cast<size_t>(rot) + kQnWarps * D) * sizeof(float);
   launch_pdl(qkv_norm_post_kernel, dim3(T), dim3(kQnWarps * 32), smem, st, qkv, bias, q_norm, k_norm, eps, inv_freq, rot, m, q_out,
              kc, vc, heads, kv_heads, D, block_size, qkv_stride, q_stride);
