@@ -17,124 +17,146 @@ namespace {
 constexpr int kQnWarps = 8;   // of qkv_norm_post_kernel
 constexpr int kQnRounds = 4;  // heads of a warp in flight in qkv_norm_vec_kernel
 
-// cos and sin of pos * inv_freq. The product is exact in float64 and reduced there: its float32
-// rounding alone would be off by 4e-3 rad at position 131072. What is left, at most pi, rounds to
-// float32 within 2^-23.
+// cos and sin of pos * inv_freq. The product is exact in float64 and reduced there, in units of pi: its float32
+// rounding alone would be off by 4e-3 rad at position 131072. What is left, at most 1, rounds to float32
+// within 2^-24 of itself.
 __device__ __forceinline__ void rotation(int pos, float inv_freq, float& c, float& s) {
-  constexpr double kTwoPi = 6.283185307179586476925;
-  const double a = static_cast<double>(pos) * static_cast<double>(inv_freq);
-  const double r = fma(-rint(a * (1.0 / kTwoPi)), kTwoPi, a);
-  sincosf(static_cast<float>(r), &s, &c);
+  constexpr double kInvTwoPi = 0.15915494309189533577;
+  const double turns = static_cast<double>(pos) * static_cast<double>(inv_freq) * kInvTwoPi;
+  sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
 }
 
 // One CTA per token. A head is held by LPH lanes, lane l with the vectors (4 values) l and, with NV = 2,
 // l + LPH; a warp takes 32 / LPH heads at a time and has U such rounds in flight, so that a token's
-// whole row is under way before anything waits: with 12 warps 24 KB at 32 + 2 x 8 heads of 128. The
-// rotation angles and the page lookup (three dependent loads) run under those loads. The partner of
-// a rotated vector is rot/8 vectors away, in another lane: it comes by shuffle.
-template <int LPH, int NV>
-__global__ void __launch_bounds__(512)
+// whole row is under way before anything waits. The rotation angles and the page lookup (three
+// dependent loads) run under those loads. The partner of a rotated vector is rot/8 vectors away, in
+// another lane: it comes by shuffle.
+// FULL: every lane holds values (head_dim = 4 LPH NV) and the whole head is rotated.
+template <int LPH, int NV, bool FULL>
+__global__ void __launch_bounds__(512, 2)
 qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const float* __restrict__ q_norm,
                     const float* __restrict__ k_norm, float eps, const float* __restrict__ inv_freq, int rot, TokenMeta m,
                     float* q_out, __half* __restrict__ kc, __half* __restrict__ vc, int heads, int kv_heads, int D, int bs,
                     int qkv_stride, int q_stride) {
-  constexpr int HPW = 32 / LPH, U = kQnRounds;
-  extern __shared__ float sm[];  // [rot/2] cos, [rot/2] sin
+  constexpr int HPW = 32 / LPH, U = kQnRounds / NV;
+  if constexpr (FULL) D = rot = 4 * LPH * NV;
+  extern __shared__ float sm[];  // [rot/2] cos, [rot/2] -sin, [rot/2] sin
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x, half = rot >> 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int sub = lane / LPH, l = lane % LPH;
+  const int sub = lane / LPH, l = lane % LPH, step = warps * HPW;
   const int vecs = D >> 2, h4 = rot >> 3;  // vectors of a head; how far a rotated vector's partner is
   const int total = heads + 2 * kv_heads;
   const int seq = m.seq[t], p = m.pos[t];
-  const float* src = qkv + static_cast<long long>(t) * qkv_stride;
-  float* dst = q_out + static_cast<long long>(t) * q_stride;
-  long long block = 0;
-  int slot = 0;
-  float4 wq[NV], wk[NV];
-  for (int h0 = 0; h0 < total; h0 += warps * HPW * U) {
+  const float* src = qkv + static_cast<long long>(t) * qkv_stride + l * 4;
+  float* dst = q_out + static_cast<long long>(t) * q_stride + l * 4;
+  const float inv_d = 1.0f / static_cast<float>(D);
+  long long page = 0;       // first value of the token's slot in KV head 0
+  float4 cs[NV], sn[NV];    // this lane's angles: y = x cos + partner * (-sin or sin)
+  for (int h0 = warp * HPW + sub; h0 - sub < total; h0 += step * U) {
     float4 x[U][NV];
-    int head[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = h0 + (u * warps + warp) * HPW + sub;
-      head[u] = h;
+      const int h = h0 + u * step;
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int v = l + n * LPH;
-        x[u][n] = h < total && v < vecs ? *reinterpret_cast<const float4*>(src + h * D + v * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+      for (int n = 0; n < NV; ++n)
+        x[u][n] = h < total && (FULL || l + n * LPH < vecs) ? *reinterpret_cast<const float4*>(src + h * D + n * LPH * 4)
+                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (h0 == 0) {
+    if (h0 < step) {  // the first time round, which every warp makes
       if (seq < 0 || p < 0) return;  // padding; looked at only here so that the row's loads do not wait for it
-      for (int i = threadIdx.x; i < half; i += blockDim.x) rotation(p, inv_freq[i], sm[i], sm[half + i]);
-      block = m.tables[m.table_off[seq] + p / bs];
-      slot = p % bs;
+      for (int i = threadIdx.x; i < half; i += blockDim.x) {
+        float c, s;
+        rotation(p, inv_freq[i], c, s);
+        sm[i] = c;
+        sm[half + i] = -s;
+        sm[2 * half + i] = s;
+      }
+      const int entry = p / bs;
+      page = (static_cast<long long>(m.tables[m.table_off[seq] + entry]) * kv_heads * bs + (p - entry * bs)) * D;
+      __syncthreads();
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int v = l + n * LPH;
-        wq[n] = q_norm && v < vecs ? reinterpret_cast<const float4*>(q_norm)[v] : make_float4(1.f, 1.f, 1.f, 1.f);
-        wk[n] = k_norm && v < vecs ? reinterpret_cast<const float4*>(k_norm)[v] : make_float4(1.f, 1.f, 1.f, 1.f);
+        cs[n] = make_float4(1.f, 1.f, 1.f, 1.f), sn[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (FULL || v < 2 * h4) {
+          const int i = (v < h4 ? v : v - h4) * 4;
+          cs[n] = *reinterpret_cast<const float4*>(sm + i);
+          sn[n] = *reinterpret_cast<const float4*>(sm + (v < h4 ? half : 2 * half) + i);
+        }
       }
-      __syncthreads();
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = head[u];
-      const bool is_q = h < heads, is_v = h >= heads + kv_heads;
-      float ss = 0.f;
+      const int h = h0 + u * step;
+      if (h - sub >= total) break;  // no head of this warp
+      const bool is_q = h < heads, is_v = h >= heads + kv_heads, there = h < total;
+      if (bias && there) {
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int v = l + n * LPH;
-        if (bias && h < total && v < vecs) {
-          const float4 b = *reinterpret_cast<const float4*>(bias + h * D + v * 4);
-          x[u][n].x += b.x, x[u][n].y += b.y, x[u][n].z += b.z, x[u][n].w += b.w;
-        }
-        ss += x[u][n].x * x[u][n].x + x[u][n].y * x[u][n].y + x[u][n].z * x[u][n].z + x[u][n].w * x[u][n].w;
+        for (int n = 0; n < NV; ++n)
+          if (FULL || l + n * LPH < vecs) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + h * D + (l + n * LPH) * 4);
+            x[u][n].x += b.x, x[u][n].y += b.y, x[u][n].z += b.z, x[u][n].w += b.w;
+          }
       }
+      if (HPW > 1 || !is_v) {  // with one head to a warp the branch is the warp's
+        const float* w = is_q ? q_norm : (is_v ? nullptr : k_norm);
+        if (q_norm || k_norm) {
+          float ss = 0.f;
 #pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (!is_v && (is_q ? q_norm : k_norm)) {
-        const float scale = 1.0f / sqrtf(ss / static_cast<float>(D) + eps);
+          for (int n = 0; n < NV; ++n)
+            ss += x[u][n].x * x[u][n].x + x[u][n].y * x[u][n].y + x[u][n].z * x[u][n].z + x[u][n].w * x[u][n].w;
+#pragma unroll
+          for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (w) {
+            const float scale = rsqrtf(ss * inv_d + eps);
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+              if (FULL || l + n * LPH < vecs) {
+                const float4 g = reinterpret_cast<const float4*>(w)[l + n * LPH];
+                x[u][n].x *= scale * g.x, x[u][n].y *= scale * g.y, x[u][n].z *= scale * g.z, x[u][n].w *= scale * g.w;
+              }
+          }
+        }
+        float4 z[NV];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-          const float4 w = is_q ? wq[n] : wk[n];
-          x[u][n].x *= scale * w.x, x[u][n].y *= scale * w.y, x[u][n].z *= scale * w.z, x[u][n].w *= scale * w.w;
+          // the partner of vector v: v + h4 for the first h4 vectors, v - h4 for the next h4
+          if constexpr (FULL && NV == 2) {
+            z[n] = x[u][1 - n];
+          } else {
+            const int v = l + n * LPH, pv = v < h4 ? v + h4 : v - h4;
+            const int from = FULL ? lane ^ (LPH / 2) : sub * LPH + (pv & (LPH - 1));
+            z[n].x = __shfl_sync(0xffffffffu, x[u][0].x, from), z[n].y = __shfl_sync(0xffffffffu, x[u][0].y, from);
+            z[n].z = __shfl_sync(0xffffffffu, x[u][0].z, from), z[n].w = __shfl_sync(0xffffffffu, x[u][0].w, from);
+            if constexpr (NV == 2) {
+              const float4 z1 = make_float4(__shfl_sync(0xffffffffu, x[u][1].x, from), __shfl_sync(0xffffffffu, x[u][1].y, from),
+                                            __shfl_sync(0xffffffffu, x[u][1].z, from), __shfl_sync(0xffffffffu, x[u][1].w, from));
+              if (pv >= LPH) z[n] = z1;
+            }
+          }
+        }
+        if (!is_v) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            if (!FULL && l + n * LPH >= 2 * h4) continue;  // passes: its "partner" may hold anything
+            x[u][n].x = x[u][n].x * cs[n].x + z[n].x * sn[n].x, x[u][n].y = x[u][n].y * cs[n].y + z[n].y * sn[n].y;
+            x[u][n].z = x[u][n].z * cs[n].z + z[n].z * sn[n].z, x[u][n].w = x[u][n].w * cs[n].w + z[n].w * sn[n].w;
+          }
         }
       }
-      float4 y[NV];
+      if (!there) continue;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        // vector v of the head and its partner: v + h4 for the first h4 vectors, v - h4 for the next h4
-        const int v = l + n * LPH, pv = v < h4 ? v + h4 : v - h4;
-        const int from = sub * LPH + (pv & (LPH - 1));
-        float4 z;
-        z.x = __shfl_sync(0xffffffffu, x[u][0].x, from), z.y = __shfl_sync(0xffffffffu, x[u][0].y, from);
-        z.z = __shfl_sync(0xffffffffu, x[u][0].z, from), z.w = __shfl_sync(0xffffffffu, x[u][0].w, from);
-        if constexpr (NV == 2) {
-          const float4 z1 = make_float4(__shfl_sync(0xffffffffu, x[u][1].x, from), __shfl_sync(0xffffffffu, x[u][1].y, from),
-                                        __shfl_sync(0xffffffffu, x[u][1].z, from), __shfl_sync(0xffffffffu, x[u][1].w, from));
-          if (pv >= LPH) z = z1;
+        if (!FULL && l + n * LPH >= vecs) continue;
+        if (is_q) {
+          *reinterpret_cast<float4*>(dst + h * D + n * LPH * 4) = x[u][n];
+        } else {
+          const int kvh = is_v ? h - heads - kv_heads : h - heads;
+          *reinterpret_cast<uint2*>((is_v ? vc : kc) + page + kvh * bs * D + (l + n * LPH) * 4) =
+              make_uint2(pack_half2(x[u][n].x, x[u][n].y), pack_half2(x[u][n].z, x[u][n].w));
         }
-        y[n] = x[u][n];
-        if (!is_v && v < 2 * h4) {
-          const int i = (v < h4 ? v : pv) * 4;
-          const float4 c = *reinterpret_cast<const float4*>(sm + i), sn = *reinterpret_cast<const float4*>(sm + half + i);
-          const float g = v < h4 ? -1.f : 1.f;
-          y[n].x = x[u][n].x * c.x + g * (z.x * sn.x), y[n].y = x[u][n].y * c.y + g * (z.y * sn.y);
-          y[n].z = x[u][n].z * c.z + g * (z.z * sn.z), y[n].w = x[u][n].w * c.w + g * (z.w * sn.w);
-        }
-      }
-      if (h >= total) continue;
-      const int kvh = is_v ? h - heads - kv_heads : h - heads;
-      __half* page = (is_v ? vc : kc) + ((block * kv_heads + kvh) * bs + slot) * D;
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int v = l + n * LPH;
-        if (v >= vecs) continue;
-        if (is_q) *reinterpret_cast<float4*>(dst + h * D + v * 4) = y[n];
-        else *reinterpret_cast<uint2*>(page + v * 4) = make_uint2(pack_half2(y[n].x, y[n].y), pack_half2(y[n].z, y[n].w));
       }
     }
   }
@@ -201,11 +223,18 @@ void launch_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, c
   auto aligned = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   if (D % 4 == 0 && rot % 8 == 0 && qkv_stride % 4 == 0 && q_stride % 4 == 0 && aligned(qkv, 16) && aligned(q_out, 16) &&
       aligned(bias, 16) && aligned(q_norm, 16) && aligned(k_norm, 16) && aligned(kc, 8) && aligned(vc, 8)) {
-    const int lanes = D > 64 ? 32 : (D > 32 ? 16 : 8);
-    const int warps = std::min(16, std::max(1, div_up(heads + 2 * kv_heads, 32 / lanes * kQnRounds)));
-    auto kernel = D > 128 ? qkv_norm_vec_kernel<32, 2>
-                          : (lanes == 32 ? qkv_norm_vec_kernel<32, 1> : (lanes == 16 ? qkv_norm_vec_kernel<16, 1> : qkv_norm_vec_kernel<8, 1>));
-    launch_pdl(kernel, dim3(T), dim3(warps * 32), rot * sizeof(float), st, qkv, bias, q_norm, k_norm, eps, inv_freq, rot, m, q_out, kc, vc,
+    const int lanes = D > 64 ? 32 : (D > 32 ? 16 : 8), nv = D > 128 ? 2 : 1;
+    // A few tokens: a warp for every kQnRounds rounds, the shortest way through. Many: at most eight warps, so that
+    // more tokens are under way on an SM (8 x 2048 tokens at 32 + 2 x 8 heads of 128: 139 us with 8 warps, 169
+    // with 12; 256 tokens: 4.9 and 3.6 us).
+    const int rounds = div_up(heads + 2 * kv_heads, 32 / lanes);
+    const int warps = T > 2 * sm_count() ? std::min(8, rounds) : std::min(16, div_up(rounds, kQnRounds / nv));
+    const bool full = rot == D && D == 4 * lanes * nv;
+    auto kernel = nv == 2       ? (full ? qkv_norm_vec_kernel<32, 2, true> : qkv_norm_vec_kernel<32, 2, false>)
+                  : lanes == 32 ? (full ? qkv_norm_vec_kernel<32, 1, true> : qkv_norm_vec_kernel<32, 1, false>)
+                  : lanes == 16 ? (full ? qkv_norm_vec_kernel<16, 1, true> : qkv_norm_vec_kernel<16, 1, false>)
+                                : (full ? qkv_norm_vec_kernel<8, 1, true> : qkv_norm_vec_kernel<8, 1, false>);
+    launch_pdl(kernel, dim3(T), dim3(warps * 32), rot / 2 * 3 * sizeof(float), st, qkv, bias, q_norm, k_norm, eps, inv_freq, rot, m, q_out, kc, vc,
                heads, kv_heads, D, block_size, qkv_stride, q_stride);
     return;
   }
