@@ -1,12 +1,12 @@
 // What a request asks of its logits ahead of the sampler: penalties for tokens that occur in its
 // history, biases, and a grammar's mask, in one pass over the row.
 //
-// A CTA owns a segment of one row's vocabulary. It counts the history's tokens of that segment in
-// shared memory (integer atomics: the counts do not depend on their order) while the segment's
-// logits are on their way into registers, then adjusts and stores them. The few biases follow as a
-// correction of what was stored, with the counters' memory now holding the last entry of each biased
-// token. 8 bytes per logit move, plus one bit of mask: the kernel is bound by memory, and by latency
-// for a few rows.
+// A CTA owns a segment of one row's vocabulary. What the mask leaves of its logits goes to registers (a vector
+// of four that the mask takes whole is not read) while the history's tokens of the segment are counted in
+// shared memory: integer atomics, so the counts do not depend on their order. Then each value is adjusted
+// and stored. The few biases follow as a correction of what was stored, with the counters' memory
+// now holding the last entry of each biased token. At most 8 bytes per logit move, plus one bit of mask:
+// the kernel is bound by memory, and by latency for a few rows.
 #include "kernels.h"
 
 namespace rb200 {
@@ -27,21 +27,19 @@ struct LogitArgs {
   int ld_logits, ld_out, V, ld_history, ld_bias, ld_mask;
 };
 
-__device__ __forceinline__ float adjusted(float x, uint32_t c, const rb200_penalties& pen) {
-  if (c) {
-    x = x > 0.0f ? x / pen.repetition : x * pen.repetition;
-    const uint32_t times = c & ~kSeen;
-    if (times) x -= pen.frequency * static_cast<float>(times) + pen.presence;
-  }
-  return x;
+// `inverse`: 1 / repetition. The product with it may differ from the quotient in the last place.
+__device__ __forceinline__ float adjusted(float x, uint32_t c, const rb200_penalties& pen, float inverse) {
+  const float times = static_cast<float>(c & ~kSeen);
+  const float less = times > 0.0f ? pen.frequency * times + pen.presence : 0.0f;
+  return c ? x * (x > 0.0f ? inverse : pen.repetition) - less : x;
 }
 
 __device__ __forceinline__ bool allowed(const uint32_t* mask, int v) { return mask == nullptr || ((mask[v >> 5] >> (v & 31)) & 1u); }
 
-// NV vectors of 4 logits per thread: a segment of 2048 NV tokens. Segments are cut on the 16-byte grid of the
-// row's memory, so the row's first `shift` (0..3) places of segment 0 lie ahead of the row.
+// NV vectors of 4 logits per thread: a segment of 4 kLgThreads NV tokens. Segments are cut on the 16-byte grid
+// of the row's memory, so the row's first `shift` (0..3) places of segment 0 lie ahead of the row.
 template <int NV>
-__global__ void __launch_bounds__(kLgThreads)
+__global__ void __launch_bounds__(kLgThreads, 1024 / kLgThreads)
 adjust_logits_kernel(const LogitArgs a) {
   constexpr int kSegment = kLgThreads * 4 * NV;
   extern __shared__ uint32_t count[];  // [kSegment]
@@ -53,114 +51,134 @@ adjust_logits_kernel(const LogitArgs a) {
   const uint32_t* mask = a.mask ? a.mask + r * a.ld_mask : nullptr;
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
   const bool same_grid = static_cast<int>((reinterpret_cast<uintptr_t>(o) >> 2) & 3) == shift;
+  const bool in_place = x == o;
   const int V = a.V, v0 = static_cast<int>(blockIdx.x) * kSegment - shift;  // token at place 0
   if (v0 >= V) return;
   const int room = min(kSegment, V - v0);  // places behind the row's end count nothing
+  const int tid = static_cast<int>(threadIdx.x);
 
-  float4 val[NV];
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int v = v0 + (n * kLgThreads + static_cast<int>(threadIdx.x)) * 4;
-    if (v >= 0 && v + 4 <= V) {
-      val[n] = *reinterpret_cast<const float4*>(x + v);
-    } else {
-      val[n].x = v >= 0 && v < V ? x[v] : 0.0f;
-      val[n].y = v + 1 >= 0 && v + 1 < V ? x[v + 1] : 0.0f;
-      val[n].z = v + 2 >= 0 && v + 2 < V ? x[v + 2] : 0.0f;
-      val[n].w = v + 3 >= 0 && v + 3 < V ? x[v + 3] : 0.0f;
-    }
-  }
-
+  // What is small and decides what follows: all of it under way before anything waits.
   rb200_penalties pen{1.0f, 0.0f, 0.0f, 0.0f};
-  bool counted = false;  // some token of the row is penalised: the same answer in every thread
+  int len = 0, prompt = 0, biases = 0;  // the same in every thread
   if (a.penalties) {
     pen = a.penalties[r];
-    const int len = min(a.history_len[r], a.ld_history);
-    counted = len > 0 && !(pen.repetition == 1.0f && pen.presence == 0.0f && pen.frequency == 0.0f);
-    if (counted) {
-      uint4* zero = reinterpret_cast<uint4*>(count);
+    len = a.history_len[r];
+    if (a.prompt_len) prompt = a.prompt_len[r];
+  }
+  if (a.bias_ids) biases = a.bias_len[r];
+
+  // Which values are in the row and pass the mask, four bits for each vector, and the values. A segment that lies
+  // inside the row on the mask's own grid needs no look at the row's ends.
+  const bool inside = shift == 0 && v0 + kSegment <= V;
+  uint32_t keep = 0;
+  float4 val[NV];
+  if (inside) {
+    uint32_t word[NV];
 #pragma unroll
-      for (int n = 0; n < NV; ++n) zero[n * kLgThreads + threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
-      __syncthreads();
-      const int prompt = a.prompt_len ? a.prompt_len[r] : 0;
-      const int* h = a.history + r * a.ld_history;
-      constexpr int U = 8;
-      for (int i0 = threadIdx.x; i0 < len; i0 += U * kLgThreads) {
-        int id[U];
+    for (int n = 0; n < NV; ++n) word[n] = mask ? mask[(v0 >> 5) + n * (kLgThreads / 8) + (tid >> 3)] : 0xffffffffu;
 #pragma unroll
-        for (int u = 0; u < U; ++u) id[u] = i0 + u * kLgThreads < len ? h[i0 + u * kLgThreads] : -1;
+    for (int n = 0; n < NV; ++n) {
+      const uint32_t bits = (word[n] >> ((tid & 7) * 4)) & 15u;
+      keep |= bits << (4 * n);
+      val[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (bits) val[n] = *reinterpret_cast<const float4*>(x + v0 + (n * kLgThreads + tid) * 4);
+    }
+  } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int at = id[u] - v0;  // ids below 0 are passed over first: the difference then fits
-          if (id[u] >= 0 && at >= 0 && at < room) {
-            if (i0 + u * kLgThreads < prompt) atomicOr(&count[at], kSeen);
-            else atomicAdd(&count[at], 1u);
-          }
-        }
+    for (int n = 0; n < NV; ++n) {
+      const int v = v0 + (n * kLgThreads + tid) * 4;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v + e >= 0 && v + e < V && allowed(mask, v + e)) bits |= 1u << e;
+      keep |= bits << (4 * n);
+      val[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (v >= 0 && v + 4 <= V) {
+        if (bits) val[n] = *reinterpret_cast<const float4*>(x + v);
+      } else {
+        if (bits & 1u) val[n].x = x[v];
+        if (bits & 2u) val[n].y = x[v + 1];
+        if (bits & 4u) val[n].z = x[v + 2];
+        if (bits & 8u) val[n].w = x[v + 3];
       }
-      __syncthreads();
     }
   }
 
+  // The place in the segment of a token id, or -1.
+  auto place = [&](int id) {
+    const int at = id - v0;  // ids below 0 are passed over first: for the others the difference fits
+    return id >= 0 && at >= 0 && at < room ? at : -1;
+  };
+  len = min(len, a.ld_history);
+  if (pen.repetition == 1.0f && pen.presence == 0.0f && pen.frequency == 0.0f) len = 0;
+  const bool counted = len > 0;
+  if (counted) {
+    const int* h = a.history + r * a.ld_history;
+    uint4* zero = reinterpret_cast<uint4*>(count);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) zero[n * kLgThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
+    constexpr int U = 8;
+    for (int i0 = tid; i0 - tid < len; i0 += U * kLgThreads) {
+      int id[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) id[u] = i0 + u * kLgThreads < len ? h[i0 + u * kLgThreads] : -1;
+      if (i0 == tid) __syncthreads();  // the counters are zero
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = place(id[u]);
+        if (at < 0) continue;
+        if (i0 + u * kLgThreads < prompt) atomicOr(&count[at], kSeen);
+        else atomicAdd(&count[at], 1u);
+      }
+    }
+    __syncthreads();
+  }
+
+  const float inverse = 1.0f / pen.repetition;
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    const int at = (n * kLgThreads + static_cast<int>(threadIdx.x)) * 4, v = v0 + at;
-    float y[4] = {val[n].x, val[n].y, val[n].z, val[n].w};
+    const int at = (n * kLgThreads + tid) * 4, v = v0 + at;
+    const uint32_t bits = keep >> (4 * n) & 15u;
+    bool changed = !in_place || bits != 15u;
     if (counted) {
       const uint4 c = *reinterpret_cast<const uint4*>(count + at);
       if (c.x | c.y | c.z | c.w) {
-        y[0] = adjusted(y[0], c.x, pen), y[1] = adjusted(y[1], c.y, pen);
-        y[2] = adjusted(y[2], c.z, pen), y[3] = adjusted(y[3], c.w, pen);
+        changed = true;
+        val[n].x = adjusted(val[n].x, c.x, pen, inverse), val[n].y = adjusted(val[n].y, c.y, pen, inverse);
+        val[n].z = adjusted(val[n].z, c.z, pen, inverse), val[n].w = adjusted(val[n].w, c.w, pen, inverse);
       }
     }
-    if (v >= 0 && v + 4 <= V) {
-      if (mask) {
-        if (shift == 0) {
-          const uint32_t bits = mask[v >> 5] >> (v & 31);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!((bits >> e) & 1u)) y[e] = -INFINITY;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!allowed(mask, v + e)) y[e] = -INFINITY;
-        }
-      }
-      if (same_grid) {
-        *reinterpret_cast<float4*>(o + v) = make_float4(y[0], y[1], y[2], y[3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[v + e] = y[e];
-      }
+    if (!changed) continue;
+    const float y[4] = {bits & 1u ? val[n].x : -INFINITY, bits & 2u ? val[n].y : -INFINITY, bits & 4u ? val[n].z : -INFINITY,
+                        bits & 8u ? val[n].w : -INFINITY};
+    if (same_grid && (inside || (v >= 0 && v + 4 <= V))) {
+      *reinterpret_cast<float4*>(o + v) = make_float4(y[0], y[1], y[2], y[3]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (v + e >= 0 && v + e < V) o[v + e] = allowed(mask, v + e) ? y[e] : -INFINITY;
+        if (v + e >= 0 && v + e < V) o[v + e] = y[e];
     }
   }
 
-  if (a.bias_ids == nullptr) return;
-  const int len = min(a.bias_len[r], a.ld_bias);
-  if (len <= 0) return;
+  biases = min(biases, a.ld_bias);
+  if (biases <= 0) return;
   const int* ids = a.bias_ids + r * a.ld_bias;
   const float* values = a.bias_values + r * a.ld_bias;
-  auto place = [&](int i) {  // of entry i in the segment, or -1
-    const int id = ids[i], at = id - v0;
-    return id >= 0 && at >= 0 && at < room ? at : -1;
-  };
-  __syncthreads();  // the counters are read, the segment is stored
-  for (int i = threadIdx.x; i < len; i += kLgThreads) {
-    const int at = place(i);
-    if (at >= 0) count[at] = 0;
+  bool any = false;
+  for (int i = tid; i < biases; i += kLgThreads) any |= place(ids[i]) >= 0;
+  if (!__syncthreads_or(any)) return;  // also: the counters are read, the segment is stored
+  for (int i = tid; i < biases; i += kLgThreads) {
+    const int at = place(ids[i]);
+    if (at >= 0) count[at] = 0u;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < len; i += kLgThreads) {
-    const int at = place(i);
+  for (int i = tid; i < biases; i += kLgThreads) {
+    const int at = place(ids[i]);
     if (at >= 0) atomicMax(&count[at], static_cast<uint32_t>(i));
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < len; i += kLgThreads) {
-    const int at = place(i);
+  for (int i = tid; i < biases; i += kLgThreads) {
+    const int at = place(ids[i]);
     if (at >= 0 && count[at] == static_cast<uint32_t>(i) && allowed(mask, v0 + at)) o[v0 + at] += values[i];
   }
 }
