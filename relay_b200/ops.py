@@ -24,6 +24,11 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _raw_stream(device: int) -> int:
+    # the current stream's handle without building a torch.cuda.Stream for it (3 us a call)
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def _dev_i32(a, device) -> torch.Tensor:
     return torch.as_tensor(a, dtype=torch.int32).to(device).contiguous()
 
@@ -86,32 +91,44 @@ def decode_attention_static(shape: CAttnShape, q, meta: TokenMeta, decode_tokens
     return out
 
 
-def _check_tensors(op: str, *named) -> None:
-    """Each (name, tensor, dtype) has that type and contiguous rows and lies on the current CUDA device; None passes."""
-    here = None
+def _here(op: str, name: str, t: torch.Tensor) -> int:
+    """The current CUDA device, which an operator's tensors have to be on; `t` is the first of them."""
+    if not t.is_cuda:
+        raise ValueError(f"{op}: {name} must be on the current CUDA device, not on {t.device}")
+    return torch.cuda.current_device()
+
+
+def _check_tensors(op: str, here: int, *named) -> None:
+    """Each (name, tensor, dtype) has that type and contiguous rows and lies on device `here`; None passes."""
     for name, t, dtype in named:
         if t is None:
             continue
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise ValueError(f"{op}: {name} must be {dtype}, not {t.dtype}")
-        if not t.is_cuda:
-            raise ValueError(f"{op}: {name} must be on the current CUDA device, not on {t.device}")
-        if here is None:
-            here = torch.cuda.current_device()
         if t.get_device() != here:
             raise ValueError(f"{op}: {name} must be on the current CUDA device {here}, not on {t.device}")
-        if t.dim() and t.size(-1) > 1 and t.stride(-1) != 1:
+        if not t.is_contiguous() and t.size(-1) > 1 and t.stride(-1) != 1:
             raise ValueError(f"{op}: the rows of {name} must be contiguous")
 
 
+def _check_meta(op: str, here: int, meta: TokenMeta, tokens: int) -> None:
+    _check_tensors(op, here, ("pos", meta.pos, torch.int32), ("seq", meta.seq, torch.int32),
+                   ("table_off", meta.table_off, torch.int32), ("tables", meta.tables, torch.int32))
+    if meta.pos.numel() < tokens or meta.seq.numel() < tokens:
+        raise ValueError(f"{op}: the metadata must have an entry for each token")
+
+
 def _check_pools(op: str, page, k_pool, v_pool) -> None:
-    for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
-        if pool.dim() != 4 or pool.shape[1:] != page or not pool.is_contiguous():
-            raise ValueError(f"{op}: {name} must be a contiguous [blocks, kv_heads, block_size, head_dim] tensor")
+    if k_pool.shape[1:] != page or v_pool.shape[1:] != page or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+        raise ValueError(f"{op}: the pools must be contiguous [blocks, kv_heads, block_size, head_dim] tensors")
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.size(0) > 1 else max(t.stride(0), t.size(1))
+    return t.size(1) if t.is_contiguous() else t.stride(0)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def shared_prefix_scratch_bytes(shape: CAttnShape, n_decode: int, n_groups: int, max_prefix: int) -> int:
@@ -127,26 +144,25 @@ def shared_prefix_attention(shape: CAttnShape, q: torch.Tensor, meta: TokenMeta,
     are read once for the group. max_prefix / max_suffix (the longest shared part, the most keys
     behind it) only decide how the work is split. A step captured as a graph passes its own scratch."""
     op, i32, f16 = "shared_prefix_attention", torch.int32, torch.float16
-    n, n_groups, rows = decode_tokens.numel(), prefix_len.numel(), meta.pos.numel()
-    _check_tensors(op, ("q", q, torch.float32), ("decode_tokens", decode_tokens, i32), ("group_off", group_off, i32),
+    n, n_groups, rows, here = decode_tokens.numel(), prefix_len.numel(), meta.pos.numel(), _here("shared_prefix_attention", "q", q)
+    _check_tensors(op, here, ("q", q, torch.float32), ("decode_tokens", decode_tokens, i32), ("group_off", group_off, i32),
                    ("prefix_len", prefix_len, i32), ("k_pool", k_pool, f16), ("v_pool", v_pool, f16), ("out", out, f16),
-                   ("scratch", scratch, torch.uint8), ("pos", meta.pos, i32), ("seq", meta.seq, i32),
-                   ("table_off", meta.table_off, i32), ("tables", meta.tables, i32))
+                   ("scratch", scratch, torch.uint8))
+    _check_meta(op, here, meta, rows)
     _check_pools(op, (shape.kv_heads, shape.block_size, shape.head_dim), k_pool, v_pool)
     if group_off.numel() != n_groups + 1:
         raise ValueError(f"{op}: group_off must have one entry more than prefix_len")
-    if meta.seq.numel() < rows:
-        raise ValueError(f"{op}: the metadata must have a sequence for each token")
+    width = shape.heads * shape.head_dim
     for name, t, stride in (("q", q, shape.q_stride), ("out", out, shape.o_stride)):
-        if t.dim() != 2 or t.size(0) < rows or t.size(1) < shape.heads * shape.head_dim or (rows > 1 and t.stride(0) != stride):
+        if t.dim() != 2 or t.size(0) < rows or t.size(1) < width or (rows > 1 and t.stride(0) != stride):
             raise ValueError(f"{op}: {name} must have the batch's rows, {stride} values apart")
+    L, sh, m = _lib.lib(), C.byref(shape), meta.c()
     if scratch is None:
-        scratch = torch.empty(max(shared_prefix_scratch_bytes(shape, n, n_groups, max_prefix), 16), dtype=torch.uint8,
+        scratch = torch.empty(max(L.rb200_shared_prefix_scratch_bytes(sh, n, n_groups, max_prefix), 16), dtype=torch.uint8,
                               device=q.device)
-    m = meta.c()
-    _lib.check(_lib.lib().rb200_shared_prefix_attention(
-        C.byref(shape), _p(q), C.byref(m), _p(decode_tokens), n, _p(group_off), _p(prefix_len), n_groups, max_prefix, max_suffix,
-        _p(k_pool), _p(v_pool), _p(scratch), scratch.numel(), _p(out), _stream()))
+    _lib.check(L.rb200_shared_prefix_attention(
+        sh, q.data_ptr(), C.byref(m), decode_tokens.data_ptr(), n, group_off.data_ptr(), prefix_len.data_ptr(), n_groups, max_prefix,
+        max_suffix, k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), out.data_ptr(), _raw_stream(here)))
     return out
 
 
@@ -223,27 +239,26 @@ def qkv_norm_post(qkv, bias, q_norm, k_norm, eps, inv_freq, meta: TokenMeta, q_o
     """qkv_post with an RMS norm over each query and key head (q_norm, k_norm [head_dim], or None) ahead of
     the rotation of its first rot_dim values (default: all): q to q_out (which may be qkv), k and v to
     their pages. A token with seq or pos below 0 is padding."""
-    op, f32, f16, i32 = "qkv_norm_post", torch.float32, torch.float16, torch.int32
-    rot = head_dim if rot_dim is None else rot_dim
-    _check_tensors(op, ("qkv", qkv, f32), ("bias", bias, f32), ("q_norm", q_norm, f32), ("k_norm", k_norm, f32),
-                   ("inv_freq", inv_freq, f32), ("q_out", q_out, f32), ("k_pool", k_pool, f16), ("v_pool", v_pool, f16),
-                   ("pos", meta.pos, i32), ("seq", meta.seq, i32), ("table_off", meta.table_off, i32), ("tables", meta.tables, i32))
-    _check_pools(op, (kv_heads, block_size, head_dim), k_pool, v_pool)
+    op, f32, f16 = "qkv_norm_post", torch.float32, torch.float16
+    rot, here = head_dim if rot_dim is None else rot_dim, _here("qkv_norm_post", "qkv", qkv)
+    _check_tensors(op, here, ("qkv", qkv, f32), ("bias", bias, f32), ("q_norm", q_norm, f32), ("k_norm", k_norm, f32),
+                   ("inv_freq", inv_freq, f32), ("q_out", q_out, f32), ("k_pool", k_pool, f16), ("v_pool", v_pool, f16))
     width = (heads + 2 * kv_heads) * head_dim
     if qkv.dim() != 2 or qkv.size(1) < width:
         raise ValueError(f"{op}: qkv must be [tokens, (heads + 2 kv_heads) head_dim]")
     T = qkv.size(0)
     if q_out.dim() != 2 or q_out.size(0) < T or q_out.size(1) < heads * head_dim:
         raise ValueError(f"{op}: q_out must be [tokens, heads head_dim]")
-    if meta.pos.numel() < T or meta.seq.numel() < T:
-        raise ValueError(f"{op}: the metadata must have an entry for each token")
+    _check_meta(op, here, meta, T)
+    _check_pools(op, (kv_heads, block_size, head_dim), k_pool, v_pool)
     for name, t, n in (("bias", bias, width), ("q_norm", q_norm, head_dim), ("k_norm", k_norm, head_dim), ("inv_freq", inv_freq, rot // 2)):
         if t is not None and t.numel() != n:
             raise ValueError(f"{op}: {name} must have {n} values")
     m = meta.c()
-    _lib.check(_lib.lib().rb200_qkv_norm_post(_p(qkv), _row_stride(qkv), _p(bias), _p(q_norm), _p(k_norm), eps, _p(inv_freq), rot,
-                                              C.byref(m), T, _p(q_out), _row_stride(q_out), _p(k_pool), _p(v_pool), heads, kv_heads,
-                                              head_dim, block_size, _stream()))
+    _lib.check(_lib.lib().rb200_qkv_norm_post(
+        qkv.data_ptr(), _row_stride(qkv), _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), rot, C.byref(m), T,
+        q_out.data_ptr(), _row_stride(q_out), k_pool.data_ptr(), v_pool.data_ptr(), heads, kv_heads, head_dim, block_size,
+        _raw_stream(here)))
     return q_out
 
 
@@ -282,31 +297,30 @@ def adjust_logits(logits, out, penalties=None, history=None, history_len=None, p
     of history [R][.], of which the first prompt_len are the prompt; bias_values for the first bias_len
     of bias_ids [R][.], the last entry of a token counting; and a mask [R][ceil(V / 32)] of int32 words,
     whose 0 bits become -inf. Ids outside the vocabulary are passed over."""
-    op, f32, i32 = "adjust_logits", torch.float32, torch.int32
-    _check_tensors(op, ("logits", logits, f32), ("out", out, f32), ("penalties", penalties, f32), ("history", history, i32),
+    op, f32, i32, here = "adjust_logits", torch.float32, torch.int32, _here("adjust_logits", "logits", logits)
+    _check_tensors(op, here, ("logits", logits, f32), ("out", out, f32), ("penalties", penalties, f32), ("history", history, i32),
                    ("history_len", history_len, i32), ("prompt_len", prompt_len, i32), ("bias_ids", bias_ids, i32),
                    ("bias_values", bias_values, f32), ("bias_len", bias_len, i32), ("mask", mask, i32))
     if logits.dim() != 2 or out.shape != logits.shape:
         raise ValueError(f"{op}: logits and out must both be [rows, vocabulary]")
     R, V = logits.shape
-    if penalties is not None and (history is None or history_len is None):
-        raise ValueError(f"{op}: penalties need a history")
-    if bias_ids is not None and (bias_values is None or bias_len is None or bias_ids.shape != bias_values.shape):
-        raise ValueError(f"{op}: bias_ids need values of the same shape and lengths")
     for name, t in (("history_len", history_len), ("prompt_len", prompt_len), ("bias_len", bias_len)):
         if t is not None and (t.numel() != R or not t.is_contiguous()):
             raise ValueError(f"{op}: {name} must have an entry for each row")
     for name, t in (("penalties", penalties), ("history", history), ("bias_ids", bias_ids), ("bias_values", bias_values)):
         if t is not None and (t.dim() != 2 or t.size(0) != R or not t.is_contiguous()):
             raise ValueError(f"{op}: {name} must be a contiguous tensor with the rows of logits")
-    if penalties is not None and penalties.size(1) != 4:
-        raise ValueError(f"{op}: penalties must be [rows, 4]")
+    if penalties is not None and (penalties.size(1) != 4 or history is None or history_len is None):
+        raise ValueError(f"{op}: penalties must be [rows, 4] and need a history")
+    if bias_ids is not None and (bias_values is None or bias_len is None or bias_ids.shape != bias_values.shape):
+        raise ValueError(f"{op}: bias_ids need values of the same shape and lengths")
     if mask is not None and (mask.dim() != 2 or mask.size(0) != R or mask.size(1) * 32 < V):
         raise ValueError(f"{op}: mask must be [rows, ceil(vocabulary / 32)]")
     _lib.check(_lib.lib().rb200_adjust_logits(
-        _p(logits), _row_stride(logits), _p(out), _row_stride(out), R, V, _p(penalties), _p(history),
-        0 if history is None else history.size(1), _p(history_len), _p(prompt_len), _p(bias_ids), _p(bias_values),
-        0 if bias_ids is None else bias_ids.size(1), _p(bias_len), _p(mask), 0 if mask is None else _row_stride(mask), _stream()))
+        logits.data_ptr(), _row_stride(logits), out.data_ptr(), _row_stride(out), R, V, _ptr(penalties), _ptr(history),
+        0 if history is None else history.size(1), _ptr(history_len), _ptr(prompt_len), _ptr(bias_ids), _ptr(bias_values),
+        0 if bias_ids is None else bias_ids.size(1), _ptr(bias_len), _ptr(mask), 0 if mask is None else _row_stride(mask),
+        _raw_stream(here)))
     return out
 
 

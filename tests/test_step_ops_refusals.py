@@ -101,13 +101,11 @@ def test_adjust_logits_refuses(kw, text):
     refused(logits(**kw), text)
 
 
-def test_the_python_wrappers_refuse_host_tensors_and_wrong_types():
+def test_the_python_wrappers_refuse_host_tensors():
     from relay_b200 import ops
     lg = torch.zeros(2, 100)
     with pytest.raises(ValueError, match="current CUDA device"):
         ops.adjust_logits(lg, lg)
-    with pytest.raises(ValueError, match="must be torch.float32"):
-        ops.adjust_logits(lg.half(), lg)
     i = torch.zeros(4, dtype=torch.int32)
     meta = ops.TokenMeta(i, i, i, i)
     pool = torch.zeros(1, 1, 16, 64, dtype=torch.float16)
