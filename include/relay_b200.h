@@ -395,14 +395,15 @@ int rb200_decode_attention_static(const rb200_attn_shape* s, const float* q, con
  *  - An entry of decode_tokens below 0, and every entry before group_off[0] or from
  *    group_off[n_groups] on, is padding: its row of out is left as it was. An entry without keys
  *    (pos < 0) gets zeros.
- *  - max_prefix and max_suffix (the longest shared part, the most keys behind it) only decide how
- *    the work is split over the GPU; other lengths on the device give the same results up to
+ *  - max_prefix and max_suffix (the longest shared part, the most keys behind it) size the scratch and
+ *    decide how the work is split over the GPU; other lengths on the device give the same results up to
  *    rounding. max_prefix 0: nothing is read as shared.
  *  - scratch (rb200_shared_prefix_scratch_bytes, 16-byte aligned, no initial state) holds the
- *    shared part's partial results of this call: calls that may overlap need one each.
+ *    partial results of this call: calls that may overlap need one each.
  * head_dim 16, 32, 64 or 128, at most 16 query heads per KV head; q 16-byte aligned with
  * q_stride a multiple of 4, the pools and out 16-byte aligned with o_stride a multiple of 8. */
-size_t rb200_shared_prefix_scratch_bytes(const rb200_attn_shape* s, int n_decode, int n_groups, int max_prefix);
+size_t rb200_shared_prefix_scratch_bytes(const rb200_attn_shape* s, int n_decode, int n_groups, int max_prefix,
+                                         int max_suffix);
 int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, const rb200_token_meta* m,
                                   const int32_t* decode_tokens, int n_decode, const int32_t* group_off,
                                   const int32_t* prefix_len, int n_groups, int max_prefix, int max_suffix,

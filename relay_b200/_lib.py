@@ -96,7 +96,7 @@ SIGNATURES = {
     "rb200_decode_plan": (SZ, [C.POINTER(CAttnShape), I, I, P, P]),
     "rb200_decode_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, I, P, P, P, SZ, P, P]),
     "rb200_decode_attention_static": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, I, P, P, P, P]),
-    "rb200_shared_prefix_scratch_bytes": (SZ, [C.POINTER(CAttnShape), I, I, I]),
+    "rb200_shared_prefix_scratch_bytes": (SZ, [C.POINTER(CAttnShape), I, I, I, I]),
     "rb200_shared_prefix_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, P, P, I, I, I, P, P, P, SZ, P,
                                           P]),
     "rb200_prefill_attention": (I, [C.POINTER(CAttnShape), P, C.POINTER(CTokenMeta), P, I, P, P, P, P]),

@@ -94,7 +94,7 @@ void launch_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, c
                           __half* vc, int heads, int kv_heads, int D, int block_size, cudaStream_t st);
 
 // ---- shared_prefix.cu ----
-size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix);
+size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix);
 void launch_shared_prefix_attention(const AttnShape& s, const float* q, const TokenMeta& m, const int* decode_tokens, int n_decode,
                                     const int* group_off, const int* prefix_len, int n_groups, int max_prefix, int max_suffix,
                                     const __half* kc, const __half* vc, float* scratch, __half* out, cudaStream_t st);

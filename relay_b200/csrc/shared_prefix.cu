@@ -6,14 +6,16 @@
 // with (m, l, o) the running maximum, sum and output of the softmax over the P shared keys and over
 // the s_i own ones. The shared part has the same keys for every token of the group, so it is a
 // product of matrices: (tokens x heads of a KV head) rows against P keys, each key read once per row
-// tile instead of once per token. Two kernels:
+// tile instead of once per token. Three kernels, each started under the one ahead:
 //
 //  * umma_prefix_kernel (umma_prefix.cu; head sizes 64 and 128, block sizes that are multiples of 16) or
 //    prefix_mma_kernel (the other layouts): a CTA takes 128 or 64 rows (token, head) of one group and
-//    KV head and a slice of the shared keys, and leaves a partial (m, l, o) per row;
-//  * suffix_kernel: a CTA takes one token and KV head (or a slice of its own keys, the slices
-//    as one cluster), streams the keys behind the prefix, adds the partials of the prefix and writes
-//    the output. It starts under the tail of the first kernel and waits for it only ahead of the join.
+//    KV head and a slice of the shared keys, and leaves a partial (m, l, o) per row. Bound by the
+//    tensor cores where many tokens share, by memory where few do;
+//  * suffix_kernel: a CTA takes one token and KV head and a slice of the token's own keys, and leaves a
+//    partial per head. Bound by memory. It needs nothing of the first kernel and runs beside it, on
+//    the SMs that one leaves free;
+//  * join_kernel: a warp takes one token and head and adds its partials.
 //
 // Scores take q in full (two fp16 halves, split_half2); the weights round to fp16 for the second product.
 #include "attn_tiles.cuh"
@@ -46,12 +48,12 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const uint32_t smem0 = smem_u32(smem_raw);
   pdl_wait();
-  pdl_trigger();  // behind the wait: what suffix_kernel reads early is then complete
+  pdl_trigger();  // behind the wait: what the kernels behind read early is then complete
   const int G = heads / kv_heads, kvh = blockIdx.y;
-  int g = 0, tile = 0, lo, hi;
-  if (!find_tile(gr, G, kPxRows, blockIdx.x, g, tile)) return;
-  group_bounds(gr, g, lo, hi);
-  const Prefix px = prefix_of(gr, m, g, lo, hi);
+  const RowTile rt = find_tile(gr, G, kPxRows, blockIdx.x);
+  if (rt.g < 0) return;
+  const int lo = rt.lo, hi = rt.hi, tile = rt.tile;
+  const Prefix px = prefix_of(gr, m, rt.g, lo, hi);
   const int slice = slice_of(px.keys, part.parts);
   const int k0 = blockIdx.z * slice;
   if (px.keys == 0 || k0 >= px.keys) return;
@@ -188,7 +190,7 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     if (entry[r] < 0) continue;
-    const long long at = (static_cast<long long>(entry[r]) * heads + head[r]) * part.parts + blockIdx.z;
+    const long long at = (static_cast<long long>(entry[r]) * heads + head[r]) * part.total + blockIdx.z;
     float* dst = part.o + at * D + 2 * t4;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
@@ -197,7 +199,7 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
 }
 
 // ---------------------------------------------------------------------------------------
-// Each sequence's own keys, and the join
+// Each sequence's own keys
 // ---------------------------------------------------------------------------------------
 
 constexpr int kSxWarps = 4;   // independent tile workers per CTA
@@ -210,39 +212,38 @@ constexpr size_t suffix_smem_bytes() {
 
 // CONTIG: block_size is a multiple of 16, so an aligned 16-key tile is one contiguous run of a page.
 // WIDE: more than 8 query heads per KV head (rows 8..15 of the M tile are real heads).
-// gridDim.z CTAs share the token's own keys as one cluster and join through distributed shared memory.
+// gridDim.z CTAs share the token's own keys.
 template <int D, bool CONTIG, bool WIDE>
 __global__ void __launch_bounds__(kSxWarps * 32, 2)
 suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half* __restrict__ kc, const __half* __restrict__ vc,
-              Partials px, __half* __restrict__ out, int heads, int kv_heads, int bs, int bs_shift, int q_stride, int o_stride,
-              float scale_log2e, int early) {
+              Partials part, int heads, int kv_heads, int bs, int bs_shift, int q_stride, float scale_log2e, int first) {
   constexpr int CH = D / 8;
   constexpr int TILE_HALVES = 16 * D;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ float s_m[kSxWarps][16], s_l[kSxWarps][16];
-  __shared__ float j_m[16], j_l[16];  // this CTA's (max, sum) per head
 
+  // Behind a prefix kernel, all of whose CTAs have waited for what came before them, the metadata, q and the
+  // pages are complete (and read from L2): nothing is waited for. Only the grid's last CTA waits, at its
+  // end, so that this kernel is not complete before the one ahead of it is. `first`: there is none.
+  if (first) pdl_wait();
   pdl_trigger();
-  // `early`: the kernel ahead is a prefix kernel, all of whose CTAs have waited for what came before them, so
-  // the metadata, q and the pages are complete (read from L2); only its partials have to be waited for.
-  if (!early) pdl_wait();
+  const bool last = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
   const int di = blockIdx.x, kvh = blockIdx.y, slices = gridDim.z, rank = blockIdx.z;
   const int tok = __ldcg(gr.decode_tokens + di);
-  const int g = group_of(gr, di);
-  if (tok < 0 || g < 0) {  // padding: the whole cluster leaves
-    pdl_wait();
+  const RowTile rt = group_of(gr, di);
+  if (tok < 0 || rt.g < 0) {  // padding
+    if (last) pdl_wait();
     return;
   }
-  int lo, hi;
-  group_bounds(gr, g, lo, hi);
-  const int P = prefix_of(gr, m, g, lo, hi).keys;
-  const int ctx = max(__ldcg(m.pos + tok) + 1, 0), start = min(P, ctx);
+  const int pos = __ldcg(m.pos + tok), seq = __ldcg(m.seq + tok);
+  const int P = prefix_of(gr, m, rt.g, rt.lo, rt.hi).keys;
+  const int ctx = max(pos + 1, 0), start = min(P, ctx);
+  const int* table = ctx > 0 ? m.tables + __ldcg(m.table_off + seq) : nullptr;
   // Tiles start at multiples of 16 where a tile has to be a run of a page; keys before `start` are masked.
   const int base = CONTIG ? start & ~15 : start;
   const int per = ((ctx - base + slices - 1) / slices + 15) & ~15;
   const int k0 = min(base + rank * per, ctx), k1 = min(k0 + per, ctx);
   const int ntiles = (k1 - k0 + 15) >> 4;
-  const int* table = ctx > 0 ? m.tables + __ldcg(m.table_off + __ldcg(m.seq + tok)) : nullptr;
 
   const int G = heads / kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -402,72 +403,99 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
     *reinterpret_cast<float2*>(os + gid * D + i * 8 + 2 * t4) = make_float2(o[i][0], o[i][1]);
     if constexpr (WIDE) *reinterpret_cast<float2*>(os + (gid + 8) * D + i * 8 + 2 * t4) = make_float2(o[i][2], o[i][3]);
   }
-  if (early) pdl_wait();
   __syncthreads();
 
   const float* os_all = reinterpret_cast<const float*>(smem_raw);
   constexpr int WARP_FLOATS = kSxStages * TILE_HALVES;  // ring size of one warp in floats
-  float* own = reinterpret_cast<float*>(smem_raw) + 16 * D;  // behind warp 0's own partial, where nothing is read any more
-  const int n_px = min(px.parts, P > 0 ? (P + slice_of(P, px.parts) - 1) / slice_of(P, px.parts) : 0);
-  // Adds the prefix's partials of head r, value d, in the order of the slices, and divides.
-  auto finish = [&](int r, int d, float M, float L, float acc) {
-    const long long at = (static_cast<long long>(di) * heads + kvh * G + r) * px.parts;
-    float top = M;
-    for (int p = 0; p < n_px; ++p) top = fmaxf(top, px.ml[(at + p) * 2]);
-    if (top == -INFINITY) top = 0.f;  // no key at all: the sums below are 0
-    const float e = fast_exp2(M - top);
-    acc *= e;
-    L *= e;
-    for (int p = 0; p < n_px; ++p) {
-      const float2 ml = *reinterpret_cast<const float2*>(px.ml + (at + p) * 2);
-      const float w = fast_exp2(ml.x - top);
-      acc += w * px.o[(at + p) * D + d];
-      L += w * ml.y;
-    }
-    out[static_cast<long long>(tok) * o_stride + (kvh * G + r) * D + d] = __float2half_rn(L == 0.f ? 0.f : acc / L);
-  };
-  for (int idx = threadIdx.x; idx < G * D; idx += blockDim.x) {
-    const int r = idx / D, d = idx - r * D;
+  for (int idx = threadIdx.x; idx < G * D / 4; idx += blockDim.x) {
+    const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
     float M = s_m[0][r];
 #pragma unroll
     for (int w = 1; w < kSxWarps; ++w) M = fmaxf(M, s_m[w][r]);
     const float ref = M == -INFINITY ? 0.f : M;
-    float acc = 0.f, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
 #pragma unroll
     for (int w = 0; w < kSxWarps; ++w) {
       const float e = fast_exp2(s_m[w][r] - ref);
-      acc += e * os_all[w * WARP_FLOATS + r * D + d];
+      const float4 x = *reinterpret_cast<const float4*>(os_all + w * WARP_FLOATS + r * D + d);
+      acc.x += e * x.x, acc.y += e * x.y, acc.z += e * x.z, acc.w += e * x.w;
       L += e * s_l[w][r];
     }
-    if (slices == 1) {
-      finish(r, d, M, L, acc);
-    } else {
-      own[idx] = acc;
-      if (d == 0) {
-        j_m[r] = M;
-        j_l[r] = L;
+    const long long at = (static_cast<long long>(di) * heads + kvh * G + r) * part.total + part.parts + rank;
+    *reinterpret_cast<float4*>(part.o + at * D + d) = acc;
+    if (d == 0) *reinterpret_cast<float2*>(part.ml + at * 2) = make_float2(M, L);
+  }
+  if (last) pdl_wait();
+}
+
+// ---------------------------------------------------------------------------------------
+// The join
+// ---------------------------------------------------------------------------------------
+
+constexpr int kMostParts = 64;  // slices of the shared keys, and of a token's own
+constexpr int kJoinWarps = 4;
+
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partials of a (token, head), one warp each. The
+// lanes first hold the partials' weights, then D / 4 of them at a time a partial's values, 128 / D partials
+// side by side; all in a fixed order.
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+join_kernel(TokenMeta m, Groups gr, Partials part, __half* __restrict__ out, int heads, int o_stride) {
+  constexpr int LPD = D / 4, SIDE = 32 / LPD, CHUNKS = 2 * kMostParts / 32;
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = min(blockIdx.x * kJoinWarps + warp, gr.n_decode * heads - 1);
+  const int di = pair / heads, head = pair - di * heads;
+  const int tok = __ldcg(gr.decode_tokens + di);
+  const RowTile rt = group_of(gr, di);
+  const bool live = tok >= 0 && rt.g >= 0 && pair == blockIdx.x * kJoinWarps + warp;
+  const int P = live ? prefix_of(gr, m, rt.g, rt.lo, rt.hi).keys : 0;
+  const int used = P > 0 ? (P + slice_of(P, part.parts) - 1) / slice_of(P, part.parts) : 0;  // slices of the shared keys
+  pdl_wait();
+  if (!live) return;
+  const long long base = static_cast<long long>(pair) * part.total;
+  float w[CHUNKS], top = -INFINITY, L = 0.f;
+  float2 ml[CHUNKS];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int p = c * 32 + lane;
+    ml[c] = p < part.total && (p < used || p >= part.parts) ? *reinterpret_cast<const float2*>(part.ml + (base + p) * 2)
+                                                            : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[c].x);
+  }
+  top = warp_max(top);
+  if (top == -INFINITY) top = 0.f;  // no key at all: every sum is 0
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    w[c] = fast_exp2(ml[c].x - top);
+    L += w[c] * ml[c].y;
+  }
+  L = warp_sum(L);
+  const int side = lane / LPD, d = (lane % LPD) * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int n = min(part.total - c * 32, 32);
+#pragma unroll 4
+    for (int p0 = 0; p0 < n; p0 += SIDE) {
+      const int p = c * 32 + p0 + side;
+      const float wp = __shfl_sync(0xffffffffu, w[c], (p0 + side) & 31);
+      if (p < part.total && (p < used || p >= part.parts)) {
+        const float4 x = *reinterpret_cast<const float4*>(part.o + (base + p) * D + d);
+        acc.x += wp * x.x, acc.y += wp * x.y, acc.z += wp * x.z, acc.w += wp * x.w;
       }
     }
   }
-  if (slices > 1) {
-    // CTA `rank` of the cluster finishes the heads r with r % slices == rank, reading the members in
-    // rank order: the result is the same on every run.
-    tc::cluster_sync_all();
-    for (int idx = threadIdx.x; idx < G * D; idx += blockDim.x) {
-      const int r = idx / D, d = idx - r * D;
-      if (r % slices != rank) continue;
-      float M = -INFINITY;
-      for (int p = 0; p < slices; ++p) M = fmaxf(M, tc::ld_dsmem_f32(smem_u32(&j_m[r]), p));
-      const float ref = M == -INFINITY ? 0.f : M;
-      float acc = 0.f, L = 0.f;
-      for (int p = 0; p < slices; ++p) {
-        const float e = fast_exp2(tc::ld_dsmem_f32(smem_u32(&j_m[r]), p) - ref);
-        acc += e * tc::ld_dsmem_f32(smem_u32(own + idx), p);
-        L += e * tc::ld_dsmem_f32(smem_u32(&j_l[r]), p);
-      }
-      finish(r, d, M, L, acc);
-    }
-    tc::cluster_sync_all();  // nobody leaves while a peer may still read its shared memory
+#pragma unroll
+  for (int o = LPD; o < 32; o <<= 1) {
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o), acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o), acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+  }
+  if (side == 0) {
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    *reinterpret_cast<uint2*>(out + static_cast<long long>(tok) * o_stride + head * D + d) =
+        make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
   }
 }
 
@@ -480,108 +508,103 @@ long long row_tiles(const AttnShape& s, int n_decode, int n_groups, int rows) {
   return (static_cast<long long>(n_decode) * (s.heads / s.kv_heads) + static_cast<long long>(n_groups) * (rows - 1)) / rows;
 }
 
-// Into how many slices the longest prefix is cut: the number that keeps the last SM busy for the shortest
-// time, a CTA costing its keys and as much as kSetupKeys more to start and to leave its partials.
-constexpr int kSetupKeys = 256;
-int prefix_parts(long long ctas, long long slots, int max_prefix) {
-  int best = 1;
-  long long least = -1;
-  for (int p = 1; p <= 64 && (p == 1 || max_prefix > (p - 1) * 2 * kPrefixSlice); ++p) {
-    const long long keys = (div_up(max_prefix, p) + kPrefixSlice - 1LL) / kPrefixSlice * kPrefixSlice;
-    const long long cost = (ctas * p + slots - 1) / slots * (keys + kSetupKeys);
-    if (least < 0 || cost < least) {
-      least = cost;
-      best = p;
-    }
-  }
-  return best;
-}
-
 int prefix_rows(const AttnShape& s) { return umma_prefix_usable(s) ? kUmmaPrefixRows : kPxRows; }
 
-// One CTA of the tcgen05 kernel fits an SM, two of the other.
-int parts_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix) {
-  const long long ctas = row_tiles(s, n_decode, n_groups, prefix_rows(s)) * s.kv_heads;
-  return prefix_parts(ctas, (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count(), max_prefix);
+// How a call is split: slices of the longest prefix and of a token's own keys.
+struct Plan {
+  int tiles, parts, slices;
+};
+
+// A CTA of a prefix kernel costs its keys and as much as kSetupKeys more to start and to leave its partials.
+constexpr int kSetupKeys = 256;
+
+Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
+  Plan p{0, 0, 1};
+  if (max_prefix > 0) {
+    // the number of slices that keeps the last SM busy for the shortest time; one CTA of the tcgen05 kernel fits
+    // an SM, two of the other
+    p.tiles = static_cast<int>(row_tiles(s, n_decode, n_groups, prefix_rows(s)));
+    const long long ctas = static_cast<long long>(p.tiles) * s.kv_heads, slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();
+    long long least = -1;
+    for (int n = 1; n <= kMostParts && (n == 1 || max_prefix > (n - 1) * 2 * kPrefixSlice); ++n) {
+      const long long keys = (div_up(max_prefix, n) + kPrefixSlice - 1LL) / kPrefixSlice * kPrefixSlice;
+      const long long cost = (ctas * n + slots - 1) / slots * (keys + kSetupKeys);
+      if (least < 0 || cost < least) {
+        least = cost;
+        p.parts = n;
+      }
+    }
+  }
+  // A few tokens with many keys of their own: slices of at least 128 keys, two CTAs for every SM.
+  const long long pairs = static_cast<long long>(n_decode) * s.kv_heads;
+  const long long slices = std::min<long long>(2LL * sm_count() / pairs, max_suffix / 128);
+  p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(slices, kMostParts)));
+  return p;
 }
 
 template <int D, bool CONTIG, bool WIDE>
 void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const __half* kc, const __half* vc,
-                   const Partials& px, __half* out, int slices, float scale_log2e, int early, cudaStream_t st) {
+                   const Partials& part, int slices, int first, cudaStream_t st) {
   static PerDeviceOnce once;
   auto kernel = suffix_kernel<D, CONTIG, WIDE>;
   if (once.first())
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(suffix_smem_bytes<D>())));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(gr.n_decode, s.kv_heads, slices);
-  cfg.blockDim = dim3(kSxWarps * 32);
-  cfg.dynamicSmemBytes = suffix_smem_bytes<D>();
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = slices;
-  cfg.attrs = attr;
-  cfg.numAttrs = slices > 1 ? 2 : 1;
   count_launch();
-  const int heads = s.heads, kv_heads = s.kv_heads, bs = s.block_size, shift = shift_of(s.block_size), qs = s.q_stride, os = s.o_stride;
-  RB_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, m, gr, kc, vc, px, out, heads, kv_heads, bs, shift, qs, os, scale_log2e, early));
+  launch_pdl(kernel, dim3(gr.n_decode, s.kv_heads, slices), dim3(kSxWarps * 32), suffix_smem_bytes<D>(), st, q, m, gr, kc, vc, part,
+             s.heads, s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, kLog2e / sqrtf(static_cast<float>(D)), first);
 }
 
 template <int D>
-void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, int max_prefix, int max_suffix,
-              const __half* kc, const __half* vc, Partials px, __half* out, cudaStream_t st) {
-  const float scale_log2e = kLog2e / sqrtf(static_cast<float>(D));
-  const int early = max_prefix > 0;
-  if (early) {
-    const long long tiles = row_tiles(s, gr.n_decode, gr.n_groups, prefix_rows(s));
+void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const Plan& plan, const __half* kc,
+              const __half* vc, const Partials& part, __half* out, cudaStream_t st) {
+  if (plan.parts > 0) {
     if (umma_prefix_usable(s)) {
-      launch_umma_prefix(s, q, m, gr, kc, vc, px, static_cast<int>(tiles), st);
+      launch_umma_prefix(s, q, m, gr, kc, vc, part, plan.tiles, st);
     } else {
       static PerDeviceOnce once;
       auto kernel = prefix_mma_kernel<D>;
       if (once.first())
         RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(prefix_smem_bytes<D>())));
       count_launch();
-      launch_pdl(kernel, dim3(static_cast<unsigned>(tiles), s.kv_heads, px.parts), dim3(128), prefix_smem_bytes<D>(), st, q, m, gr, kc, vc,
-                 px, s.heads, s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, scale_log2e);
+      launch_pdl(kernel, dim3(plan.tiles, s.kv_heads, plan.parts), dim3(128), prefix_smem_bytes<D>(), st, q, m, gr, kc, vc, part, s.heads,
+                 s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, kLog2e / sqrtf(static_cast<float>(D)));
     }
   }
-  // A few tokens with many keys of their own: up to eight CTAs of at least 128 keys for each (token, KV head).
-  const long long pairs = static_cast<long long>(gr.n_decode) * s.kv_heads;
-  int slices = 1;
-  while (slices < 8 && pairs * slices * 2 <= 2LL * sm_count() && max_suffix / (slices * 2) >= 128) slices *= 2;
   const bool contig = s.block_size % 16 == 0, wide = s.heads / s.kv_heads > 8;
-  if (contig && !wide) launch_suffix<D, true, false>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
-  else if (contig) launch_suffix<D, true, true>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
-  else if (!wide) launch_suffix<D, false, false>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
-  else launch_suffix<D, false, true>(s, q, m, gr, kc, vc, px, out, slices, scale_log2e, early, st);
+  const int first = plan.parts == 0;
+  if (contig && !wide) launch_suffix<D, true, false>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  else if (contig) launch_suffix<D, true, true>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  else if (!wide) launch_suffix<D, false, false>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  else launch_suffix<D, false, true>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  count_launch();
+  launch_pdl(join_kernel<D>, dim3(div_up(static_cast<long long>(gr.n_decode) * s.heads, kJoinWarps)), dim3(kJoinWarps * 32), 0, st, m, gr,
+             part, out, s.heads, s.o_stride);
 }
 
 }  // namespace
 
-size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix) {
+size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
   if (n_decode <= 0 || n_groups <= 0) return 0;
-  return static_cast<size_t>(n_decode) * s.heads * parts_of(s, n_decode, n_groups, max_prefix) * (s.D + 2) * sizeof(float);
+  const Plan p = plan_of(s, n_decode, n_groups, max_prefix, max_suffix);
+  return static_cast<size_t>(n_decode) * s.heads * (p.parts + p.slices) * (s.D + 2) * sizeof(float);
 }
 
 void launch_shared_prefix_attention(const AttnShape& s, const float* q, const TokenMeta& m, const int* decode_tokens, int n_decode,
                                     const int* group_off, const int* prefix_len, int n_groups, int max_prefix, int max_suffix,
                                     const __half* kc, const __half* vc, float* scratch, __half* out, cudaStream_t st) {
   if (n_decode == 0) return;
-  const Groups gr{decode_tokens, group_off, max_prefix > 0 ? prefix_len : nullptr, n_decode, n_groups};
-  Partials px;
-  px.parts = parts_of(s, n_decode, n_groups, max_prefix);
-  px.o = scratch;
-  px.ml = scratch + static_cast<size_t>(n_decode) * s.heads * px.parts * s.D;
+  const Plan plan = plan_of(s, n_decode, n_groups, max_prefix, max_suffix);
+  const Groups gr{decode_tokens, group_off, plan.parts > 0 ? prefix_len : nullptr, n_decode, n_groups};
+  Partials part;
+  part.parts = plan.parts;
+  part.total = plan.parts + plan.slices;
+  part.o = scratch;
+  part.ml = scratch + static_cast<size_t>(n_decode) * s.heads * part.total * s.D;
   switch (s.D) {
-    case 16: launch_d<16>(s, q, m, gr, max_prefix, max_suffix, kc, vc, px, out, st); break;
-    case 32: launch_d<32>(s, q, m, gr, max_prefix, max_suffix, kc, vc, px, out, st); break;
-    case 64: launch_d<64>(s, q, m, gr, max_prefix, max_suffix, kc, vc, px, out, st); break;
-    case 128: launch_d<128>(s, q, m, gr, max_prefix, max_suffix, kc, vc, px, out, st); break;
+    case 16: launch_d<16>(s, q, m, gr, plan, kc, vc, part, out, st); break;
+    case 32: launch_d<32>(s, q, m, gr, plan, kc, vc, part, out, st); break;
+    case 64: launch_d<64>(s, q, m, gr, plan, kc, vc, part, out, st); break;
+    case 128: launch_d<128>(s, q, m, gr, plan, kc, vc, part, out, st); break;
     default: fail(RB200_ERR_INVALID_ARGUMENT, "shared prefix attention: head_dim must be 16, 32, 64 or 128");
   }
 }
@@ -596,9 +619,9 @@ static AttnShape shape_of(const rb200_attn_shape* s) {
 
 extern "C" {
 
-size_t rb200_shared_prefix_scratch_bytes(const rb200_attn_shape* s, int n_decode, int n_groups, int max_prefix) {
-  if (!s || !fast_attention_supported(shape_of(s))) return 0;
-  return shared_prefix_scratch_bytes(shape_of(s), n_decode, n_groups, max_prefix);
+size_t rb200_shared_prefix_scratch_bytes(const rb200_attn_shape* s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
+  if (!s || !fast_attention_supported(shape_of(s)) || max_prefix < 0 || max_suffix < 0) return 0;
+  return shared_prefix_scratch_bytes(shape_of(s), n_decode, n_groups, max_prefix, max_suffix);
 }
 
 int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, const rb200_token_meta* m, const int32_t* decode_tokens,
@@ -622,7 +645,7 @@ int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, con
                "shared prefix attention: null argument");
     for (const void* p : {static_cast<const void*>(q), k_pool, v_pool, static_cast<const void*>(scratch), static_cast<const void*>(out)})
       RB_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "shared prefix attention: q, the pools, scratch and out must be 16-byte aligned");
-    RB_REQUIRE(scratch_bytes >= shared_prefix_scratch_bytes(sh, n_decode, n_groups, max_prefix),
+    RB_REQUIRE(scratch_bytes >= shared_prefix_scratch_bytes(sh, n_decode, n_groups, max_prefix, max_suffix),
                "shared prefix attention: scratch too small");
     launch_shared_prefix_attention(sh, q, TokenMeta{m->pos, m->seq, m->table_off, m->tables}, decode_tokens, n_decode, group_off,
                                    prefix_len, n_groups, max_prefix, max_suffix, static_cast<const __half*>(k_pool),

@@ -68,22 +68,7 @@ umma_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const uint32_t p_ready = bars + 176, pv_done = bars + 192;  // one per half
   const uint32_t q_ready = bars + 208, tmem_slot = bars + 216;
 
-  // Everything, the group metadata too, may come from the kernel ahead. The trigger follows the wait, so
-  // that whatever the kernel behind this one reads early is complete by the time it starts.
-  pdl_wait();
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = heads / kv_heads, kvh = blockIdx.y;
-  int g = 0, tile = 0, lo, hi;
-  if (!find_tile(gr, G, kRows, blockIdx.x, g, tile)) return;
-  group_bounds(gr, g, lo, hi);
-  const Prefix px = prefix_of(gr, m, g, lo, hi);
-  const int slice = slice_of(px.keys, part.parts);
-  const int k0 = blockIdx.z * slice;
-  if (px.keys == 0 || k0 >= px.keys) return;
-  const int k1 = min(px.keys, k0 + slice);
-  const int ntiles = (k1 - k0 + kKeys - 1) / kKeys;
-
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(full + 8 * s, 1);
@@ -99,17 +84,35 @@ umma_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
+  if (warp == 1 && lane == 0) {
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
+  // Everything, the group metadata too, may come from the kernel ahead. TMEM is taken behind the wait (a CTA that
+  // holds it and waits could keep the kernel ahead from getting its own) and the trigger comes last, so
+  // that whatever the kernels behind this one read early is complete by the time they start.
+  pdl_wait();
   if (warp == 2) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
+  const int G = heads / kv_heads, kvh = blockIdx.y;
+  const RowTile rt = find_tile(gr, G, kRows, blockIdx.x);
+  const int lo = rt.lo, hi = rt.hi, tile = rt.tile;
+  const Prefix px = rt.g >= 0 ? prefix_of(gr, m, rt.g, lo, hi) : Prefix{0, nullptr};
+  const int slice = slice_of(px.keys, part.parts);
+  const int k0 = blockIdx.z * slice, k1 = min(px.keys, k0 + slice);
+  const int ntiles = (k1 - k0 + kKeys - 1) / kKeys;  // 0 or less: nothing to do
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(gen + (tmem_slot - base));
 
   bool ok = true;
-  if (warp < 2 || warp == 3) {
+  if (ntiles <= 0) {
+    // no such tile or slice
+  } else if (warp < 2 || warp == 3) {
     // ---- loaders: a tile's keys come from 8 pages of 16 keys; one box per page and 64-wide slice of the
     //      head, dealt round-robin to the lanes of three warps. Page rows are looked up 32 at a time (four
     //      tiles), one per lane, a group ahead of their use. Pages that the slice does not fill are
@@ -355,7 +358,7 @@ umma_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const float m_b = park[row], l_b = park[kRows + row];
       const float M = fmaxf(m_ref, m_b), ref = M == -INFINITY ? 0.f : M;
       const float wa = fast_exp2(m_ref - ref), wb = fast_exp2(m_b - ref);
-      const long long at = (static_cast<long long>(entry) * heads + head) * part.parts + blockIdx.z;
+      const long long at = (static_cast<long long>(entry) * heads + head) * part.total + blockIdx.z;
       if (tok >= 0) *reinterpret_cast<float2*>(part.ml + at * 2) = make_float2(M, wa * l_run + wb * l_b);
       float* dst = part.o + at * D;
 #pragma unroll

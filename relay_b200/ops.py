@@ -131,8 +131,8 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def shared_prefix_scratch_bytes(shape: CAttnShape, n_decode: int, n_groups: int, max_prefix: int) -> int:
-    return _lib.lib().rb200_shared_prefix_scratch_bytes(C.byref(shape), n_decode, n_groups, max_prefix)
+def shared_prefix_scratch_bytes(shape: CAttnShape, n_decode: int, n_groups: int, max_prefix: int, max_suffix: int) -> int:
+    return _lib.lib().rb200_shared_prefix_scratch_bytes(C.byref(shape), n_decode, n_groups, max_prefix, max_suffix)
 
 
 def shared_prefix_attention(shape: CAttnShape, q: torch.Tensor, meta: TokenMeta, decode_tokens: torch.Tensor,
@@ -158,7 +158,7 @@ def shared_prefix_attention(shape: CAttnShape, q: torch.Tensor, meta: TokenMeta,
             raise ValueError(f"{op}: {name} must have the batch's rows, {stride} values apart")
     L, sh, m = _lib.lib(), C.byref(shape), meta.c()
     if scratch is None:
-        scratch = torch.empty(max(L.rb200_shared_prefix_scratch_bytes(sh, n, n_groups, max_prefix), 16), dtype=torch.uint8,
+        scratch = torch.empty(max(L.rb200_shared_prefix_scratch_bytes(sh, n, n_groups, max_prefix, max_suffix), 16), dtype=torch.uint8,
                               device=q.device)
     _lib.check(L.rb200_shared_prefix_attention(
         sh, q.data_ptr(), C.byref(m), decode_tokens.data_ptr(), n, group_off.data_ptr(), prefix_len.data_ptr(), n_groups, max_prefix,

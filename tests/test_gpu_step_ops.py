@@ -318,7 +318,7 @@ def test_shared_prefix_attention_agrees_with_decode_attention(ops, D, heads, kv_
 def test_shared_prefix_attention_scratch_may_hold_anything(ops):
     c = prefix_case(9, 128, 8, 2, 16, [(3000, [1, 30]), (0, [9]), (100, [4])])
     shape = ops.attn_shape(8, 2, 128, 16)
-    need = ops.shared_prefix_scratch_bytes(shape, 4, 3, c["max_prefix"])
+    need = ops.shared_prefix_scratch_bytes(shape, 4, 3, c["max_prefix"], c["max_suffix"])
     scratch = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")  # NaN in every word
     check_prefix(c, run_prefix(ops, c, scratch=scratch[:need]), 7.0)
     assert torch.all(scratch[need:] == 255)
@@ -530,7 +530,7 @@ class Step:
         self.logits = torch.zeros((T, self.V), device="cuda")
         self.picked = torch.full((T,), -1, dtype=torch.int32, device="cuda")
         self.sampling = torch.zeros((T, 32), dtype=torch.uint8, device="cuda")  # temperature 0
-        self.scratch = torch.empty(ops.shared_prefix_scratch_bytes(self.shape, T, 3, 333), dtype=torch.uint8, device="cuda")
+        self.scratch = torch.empty(ops.shared_prefix_scratch_bytes(self.shape, T, 3, 333, 77), dtype=torch.uint8, device="cuda")
 
     def run(self):
         g, o = self.g, self.ops

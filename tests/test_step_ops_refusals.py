@@ -77,10 +77,12 @@ def test_shared_prefix_scratch_is_host_computable():
     L = _lib.lib()
     sh = _lib.CAttnShape(32, 8, 128, 16, 6144, 4096)
     per = 4 * 32 * 130 * 4  # one slice of four tokens: (D + 2) floats per (token, head)
-    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 100) == per
-    many = L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 100000)
-    assert many > per and many % per == 0
-    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 0, 0, 100) == 0
+    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 100, 100) == 2 * per  # of the shared keys and of the own ones
+    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 0, 100) == per
+    for lens in ((100000, 100), (100, 100000)):
+        many = L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, *lens)
+        assert many > 2 * per and many % per == 0
+    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 0, 0, 100, 100) == 0
 
 
 def logits(**kw):
