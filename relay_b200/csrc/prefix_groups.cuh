@@ -11,8 +11,7 @@
 
 namespace rb200 {
 
-constexpr int kPrefixSlice = 128;     // slices of the shared keys are multiples of this
-constexpr int kUmmaPrefixRows = 128;  // rows (token, head) of a CTA of umma_prefix_kernel
+constexpr int kPrefixSlice = 128;  // slices of the shared keys are multiples of this
 
 // The group geometry on the device.
 struct Groups {
@@ -34,21 +33,21 @@ struct Partials {
 
 __device__ __forceinline__ int slice_of(int P, int parts) { return (((P + parts - 1) / parts) + kPrefixSlice - 1) / kPrefixSlice * kPrefixSlice; }
 
-// How many keys the entries [lo, hi) of group g share, and the block table that names them.
+// How many keys the entries [lo, hi) of group g share, and (`with_table`) the block table that names them.
 struct Prefix {
   int keys;
   const int* table;
 };
-__device__ __forceinline__ Prefix prefix_of(const Groups& gr, const TokenMeta& m, int g, int lo, int hi) {
+__device__ __forceinline__ Prefix prefix_of(const Groups& gr, const TokenMeta& m, int g, int lo, int hi, bool with_table) {
   if (gr.prefix_len == nullptr || lo >= hi) return {0, nullptr};
   const int len = __ldcg(gr.prefix_len + g);
   int tok = __ldcg(gr.decode_tokens + lo);
   for (int i = lo + 1; i < hi && tok < 0; ++i) tok = __ldcg(gr.decode_tokens + i);  // the first entry that is not padding
   if (tok < 0) return {0, nullptr};
-  const int pos = __ldcg(m.pos + tok), seq = __ldcg(m.seq + tok);
+  const int pos = __ldcg(m.pos + tok), seq = with_table ? __ldcg(m.seq + tok) : 0;
   const int keys = min(len, pos + 1);
   if (keys <= 0) return {0, nullptr};
-  return {keys, m.tables + __ldcg(m.table_off + seq)};
+  return {keys, with_table ? m.tables + __ldcg(m.table_off + seq) : nullptr};
 }
 
 // A row tile: group g, its entries [lo, hi), and the tile's number in the group.
@@ -100,9 +99,9 @@ __device__ __forceinline__ RowTile group_of(const Groups& gr, int di) {
 }
 
 // umma_prefix.cu: the shared keys on tcgen05 tensor cores, for head sizes 64 and 128 and block sizes that are
-// multiples of 16; `tiles` bounds the row tiles of kUmmaPrefixRows rows.
+// multiples of 16; `tiles` bounds the row tiles of `rows` rows (64 or 128).
 bool umma_prefix_usable(const AttnShape& s);
 void launch_umma_prefix(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const __half* kc, const __half* vc,
-                        const Partials& px, int tiles, cudaStream_t st);
+                        const Partials& px, int rows, int tiles, cudaStream_t st);
 
 }  // namespace rb200

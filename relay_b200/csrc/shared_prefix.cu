@@ -53,7 +53,7 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
   const RowTile rt = find_tile(gr, G, kPxRows, blockIdx.x);
   if (rt.g < 0) return;
   const int lo = rt.lo, hi = rt.hi, tile = rt.tile;
-  const Prefix px = prefix_of(gr, m, rt.g, lo, hi);
+  const Prefix px = prefix_of(gr, m, rt.g, lo, hi, true);
   const int slice = slice_of(px.keys, part.parts);
   const int k0 = blockIdx.z * slice;
   if (px.keys == 0 || k0 >= px.keys) return;
@@ -236,7 +236,7 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
     return;
   }
   const int pos = __ldcg(m.pos + tok), seq = __ldcg(m.seq + tok);
-  const int P = prefix_of(gr, m, rt.g, rt.lo, rt.hi).keys;
+  const int P = prefix_of(gr, m, rt.g, rt.lo, rt.hi, false).keys;
   const int ctx = max(pos + 1, 0), start = min(P, ctx);
   const int* table = ctx > 0 ? m.tables + __ldcg(m.table_off + seq) : nullptr;
   // Tiles start at multiples of 16 where a tile has to be a run of a page; keys before `start` are masked.
@@ -450,7 +450,7 @@ join_kernel(TokenMeta m, Groups gr, Partials part, __half* __restrict__ out, int
   const int tok = __ldcg(gr.decode_tokens + di);
   const RowTile rt = group_of(gr, di);
   const bool live = tok >= 0 && rt.g >= 0 && pair == blockIdx.x * kJoinWarps + warp;
-  const int P = live ? prefix_of(gr, m, rt.g, rt.lo, rt.hi).keys : 0;
+  const int P = live ? prefix_of(gr, m, rt.g, rt.lo, rt.hi, false).keys : 0;
   const int used = P > 0 ? (P + slice_of(P, part.parts) - 1) / slice_of(P, part.parts) : 0;  // slices of the shared keys
   pdl_wait();
   if (!live) return;
@@ -477,13 +477,22 @@ join_kernel(TokenMeta m, Groups gr, Partials part, __half* __restrict__ out, int
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int n = min(part.total - c * 32, 32);
-#pragma unroll 4
-    for (int p0 = 0; p0 < n; p0 += SIDE) {
-      const int p = c * 32 + p0 + side;
-      const float wp = __shfl_sync(0xffffffffu, w[c], (p0 + side) & 31);
-      if (p < part.total && (p < used || p >= part.parts)) {
-        const float4 x = *reinterpret_cast<const float4*>(part.o + (base + p) * D + d);
-        acc.x += wp * x.x, acc.y += wp * x.y, acc.z += wp * x.z, acc.w += wp * x.w;
+    constexpr int U = 8;  // loads in flight
+#pragma unroll 1
+    for (int p0 = 0; p0 < n; p0 += U * SIDE) {
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int p = c * 32 + p0 + u * SIDE + side;
+        x[u] = p < part.total && (p < used || p >= part.parts) ? *reinterpret_cast<const float4*>(part.o + (base + p) * D + d)
+                                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float wp = __shfl_sync(0xffffffffu, w[c], (p0 + u * SIDE + side) & 31);
+        const bool there = p0 + u * SIDE + side < 32;  // else the weight is another partial's
+        acc.x += there ? wp * x[u].x : 0.f, acc.y += there ? wp * x[u].y : 0.f;
+        acc.z += there ? wp * x[u].z : 0.f, acc.w += there ? wp * x[u].w : 0.f;
       }
     }
   }
@@ -508,29 +517,36 @@ long long row_tiles(const AttnShape& s, int n_decode, int n_groups, int rows) {
   return (static_cast<long long>(n_decode) * (s.heads / s.kv_heads) + static_cast<long long>(n_groups) * (rows - 1)) / rows;
 }
 
-int prefix_rows(const AttnShape& s) { return umma_prefix_usable(s) ? kUmmaPrefixRows : kPxRows; }
-
-// How a call is split: slices of the longest prefix and of a token's own keys.
+// How a call is split: row tiles, slices of the longest prefix and of a token's own keys.
 struct Plan {
-  int tiles, parts, slices;
+  int rows, tiles, parts, slices;
 };
 
-// A CTA of a prefix kernel costs its keys and as much as kSetupKeys more to start and to leave its partials.
-constexpr int kSetupKeys = 256;
+// The number of slices of the shared keys follows from an estimate of the call's time for each, in us: a CTA of
+// the prefix kernel takes kTileUs for every 128 keys and kStartUs besides; the own keys (about half of the
+// most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel
+// leaves free get kBytesPerSmUs each until it ends. 256 tokens of 32 heads behind 8192 keys with 128 - 640 of
+// their own: one slice, 64 CTAs beside the own keys, against 123 us with the two slices that fill the GPU.
+constexpr double kTileUs = 1.3, kStartUs = 6.0, kBytesPerUs = 6.0e6, kBytesPerSmUs = 5.0e4;
 
 Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
-  Plan p{0, 0, 1};
+  Plan p{0, 0, 0, 1};
+  const double own_us = 2.0 * max_suffix * s.D * s.kv_heads * n_decode / kBytesPerUs;
   if (max_prefix > 0) {
-    // the number of slices that keeps the last SM busy for the shortest time; one CTA of the tcgen05 kernel fits
-    // an SM, two of the other
-    p.tiles = static_cast<int>(row_tiles(s, n_decode, n_groups, prefix_rows(s)));
-    const long long ctas = static_cast<long long>(p.tiles) * s.kv_heads, slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();
-    long long least = -1;
+    // 64 rows where the average group has no more
+    p.rows = umma_prefix_usable(s) && static_cast<long long>(n_decode) * (s.heads / s.kv_heads) > 64LL * n_groups ? 128 : 64;
+    p.tiles = static_cast<int>(row_tiles(s, n_decode, n_groups, p.rows));
+    const long long ctas = static_cast<long long>(p.tiles) * s.kv_heads;
+    const long long slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();  // one CTA of the tcgen05 kernel fits an SM
+    double least = -1.0;
     for (int n = 1; n <= kMostParts && (n == 1 || max_prefix > (n - 1) * 2 * kPrefixSlice); ++n) {
-      const long long keys = (div_up(max_prefix, n) + kPrefixSlice - 1LL) / kPrefixSlice * kPrefixSlice;
-      const long long cost = (ctas * n + slots - 1) / slots * (keys + kSetupKeys);
-      if (least < 0 || cost < least) {
-        least = cost;
+      const double waves = static_cast<double>((ctas * n + slots - 1) / slots);
+      const double shared_us = waves * (div_up(div_up(max_prefix, n), kPrefixSlice) * kTileUs + kStartUs);
+      const double idle = std::max<double>(0.0, 1.0 - static_cast<double>(ctas * n) / slots) * sm_count();
+      const double beside = shared_us * std::min(1.0, idle * kBytesPerSmUs / kBytesPerUs);
+      const double us = shared_us + std::max(0.0, own_us - beside);
+      if (least < 0.0 || us < least) {
+        least = us;
         p.parts = n;
       }
     }
@@ -559,7 +575,7 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
               const __half* vc, const Partials& part, __half* out, cudaStream_t st) {
   if (plan.parts > 0) {
     if (umma_prefix_usable(s)) {
-      launch_umma_prefix(s, q, m, gr, kc, vc, part, plan.tiles, st);
+      launch_umma_prefix(s, q, m, gr, kc, vc, part, plan.rows, plan.tiles, st);
     } else {
       static PerDeviceOnce once;
       auto kernel = prefix_mma_kernel<D>;
