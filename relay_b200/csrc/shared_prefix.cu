@@ -523,15 +523,16 @@ struct Plan {
 };
 
 // The number of slices of the shared keys follows from an estimate of the call's time for each, in us: a CTA of
-// the prefix kernel takes kTileUs for every 128 keys and kStartUs besides; the own keys (about half of the
-// most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel
-// leaves free get kBytesPerSmUs each until it ends. 256 tokens of 32 heads behind 8192 keys with 128 - 640 of
-// their own: one slice, 64 CTAs beside the own keys, against 123 us with the two slices that fill the GPU.
-constexpr double kTileUs = 1.3, kStartUs = 6.0, kBytesPerUs = 6.0e6, kBytesPerSmUs = 5.0e4;
+// the prefix kernel takes kTileUs for every 128 keys and kStartUs besides; the own keys (six tenths of the
+// most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel leaves
+// free get kBytesPerSmUs each until it ends. Measured at 32 + 2 x 8 heads of 128: 256 tokens behind 8192 keys
+// with 128 - 640 of their own, 108 us in one slice (64 CTAs beside the own keys) and 120 in two, which fill the
+// GPU; 32 tokens behind 4096 with 64 - 512: 25, 22, 26 and 27 us in 4, 8, 11 and 16 slices.
+constexpr double kTileUs = 1.3, kStartUs = 6.0, kBytesPerUs = 5.5e6, kBytesPerSmUs = 4.2e4;
 
 Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
   Plan p{0, 0, 0, 1};
-  const double own_us = 2.0 * max_suffix * s.D * s.kv_heads * n_decode / kBytesPerUs;
+  const double own_us = 0.6 * 4.0 * max_suffix * s.D * s.kv_heads * n_decode / kBytesPerUs;
   if (max_prefix > 0) {
     // 64 rows where the average group has no more
     p.rows = umma_prefix_usable(s) && static_cast<long long>(n_decode) * (s.heads / s.kv_heads) > 64LL * n_groups ? 128 : 64;
