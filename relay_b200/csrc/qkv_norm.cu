@@ -5,9 +5,10 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)  on the pairs (i, i + rot/2) of y
 //
 // Every value is read once and written once: 4 (Q + 2 KV) bytes of a token come in, 4 Q + 4 KV go
-// out, so the kernel is bound by memory, and by latency for a few tokens. Heads whose rows are whole
-// 16-byte vectors take qkv_norm_vec_kernel, which keeps a head in the registers of 8, 16 or 32 lanes;
-// the others (head_dim not a multiple of 4, rot_dim not of 8, unaligned rows) qkv_norm_post_kernel.
+// out, so the kernels are bound by memory, and by latency for a few tokens. Heads of 32, 64, 128 or 256 values
+// that are rotated whole or by half take qkv_norm_pair_kernel; other heads whose rows are whole 16-byte
+// vectors qkv_norm_vec_kernel; the rest (head_dim not a multiple of 4, rot_dim not of 8, unaligned rows)
+// qkv_norm_post_kernel.
 #include "kernels.h"
 
 namespace rb200 {
@@ -15,7 +16,8 @@ namespace rb200 {
 namespace {
 
 constexpr int kQnWarps = 8;   // of qkv_norm_post_kernel
-constexpr int kQnRounds = 4;  // heads of a warp in flight in qkv_norm_vec_kernel
+constexpr int kQnRounds = 4;      // rounds of a warp in flight in qkv_norm_vec_kernel
+constexpr int kQnPairRounds = 2;  // and in qkv_norm_pair_kernel
 
 // cos and sin of pos * inv_freq. The product is exact in float64 and reduced there, in units of pi: its float32
 // rounding alone would be off by 4e-3 rad at position 131072. What is left, at most 1, rounds to float32
@@ -26,20 +28,130 @@ __device__ __forceinline__ void rotation(int pos, float inv_freq, float& c, floa
   sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
 }
 
+// The values of a vector as two pairs, the operands of packed fp32 instructions.
+struct Pair2 {
+  float2 a, b;
+};
+__device__ __forceinline__ Pair2 pairs(const float4& v) { return {make_float2(v.x, v.y), make_float2(v.z, v.w)}; }
+__device__ __forceinline__ Pair2 mul(const Pair2& x, const Pair2& y) { return {__fmul2_rn(x.a, y.a), __fmul2_rn(x.b, y.b)}; }
+__device__ __forceinline__ Pair2 fma(const Pair2& x, const Pair2& y, const Pair2& z) {
+  return {__ffma2_rn(x.a, y.a, z.a), __ffma2_rn(x.b, y.b, z.b)};
+}
+__device__ __forceinline__ Pair2 add(const Pair2& x, const Pair2& y) { return {__fadd2_rn(x.a, y.a), __fadd2_rn(x.b, y.b)}; }
+__device__ __forceinline__ Pair2 all(float v) { return {make_float2(v, v), make_float2(v, v)}; }
+
+// Heads of 8 LPH values. LPH lanes hold one, lane l its vectors l and l + LPH: rotated whole, a vector's partner is
+// in the same lane; rotated by half, all that turns is in the first vectors and the partner LPH / 2 lanes
+// away. A warp takes 32 / LPH heads at a time and has kQnPairRounds such rounds in flight. A CTA goes through
+// tokens a grid apart: a token's position and page (three dependent loads) are looked up while the one before
+// it is at work, its angles are computed under its row's loads. What kept a first form of this kernel (a
+// head in 32 lanes, 126 instructions a head) at 139 us for 8 x 2048 tokens was instruction issue; hence
+// two vectors a lane and packed arithmetic.
+template <int LPH, bool HALF>
+__global__ void __launch_bounds__(512, 2)
+qkv_norm_pair_kernel(const float* qkv, const float* __restrict__ bias, const float* __restrict__ q_norm,
+                     const float* __restrict__ k_norm, float eps, const float* __restrict__ inv_freq, TokenMeta m, int T, float* q_out,
+                     __half* __restrict__ kc, __half* __restrict__ vc, int heads, int kv_heads, int bs, int qkv_stride, int q_stride) {
+  constexpr int D = 8 * LPH, HPW = 32 / LPH, U = kQnPairRounds, kAngles = HALF ? D / 4 : D / 2;
+  __shared__ __align__(16) float s_cos[2][kAngles], s_sin[2][kAngles];  // tokens in turn
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int sub = lane / LPH, l = lane % LPH, step = warps * HPW, total = heads + 2 * kv_heads;
+  int t = blockIdx.x, seq = m.seq[t], p = m.pos[t], turn = 0;
+  int block = seq >= 0 && p >= 0 ? m.tables[m.table_off[seq] + p / bs] : 0;
+  while (true) {
+    const int t_next = t + gridDim.x;
+    const int seq_next = t_next < T ? m.seq[t_next] : -1, p_next = t_next < T ? m.pos[t_next] : -1;
+    const bool next = seq_next >= 0 && p_next >= 0;
+    int entry_next = -1;  // of the next token's page in the tables
+    if (seq >= 0 && p >= 0) {  // else padding
+      const float* src = qkv + static_cast<long long>(t) * qkv_stride + l * 4;
+      float* dst = q_out + static_cast<long long>(t) * q_stride + l * 4;
+      const long long page = (static_cast<long long>(block) * kv_heads * bs + p % bs) * D + l * 4;  // the slot in KV head 0
+      Pair2 c, s, ns;  // this lane's cos, sin and -sin
+      for (int h0 = warp * HPW + sub; h0 - sub < total; h0 += step * U) {
+        float4 x[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = min(h0 + u * step, total - 1);  // behind the last head: read, not written
+          x[u][0] = *reinterpret_cast<const float4*>(src + h * D);
+          x[u][1] = *reinterpret_cast<const float4*>(src + h * D + D / 2);
+        }
+        if (h0 < step) {  // the first time round, which every warp makes
+          for (int i = threadIdx.x; i < kAngles; i += blockDim.x) rotation(p, inv_freq[i], s_cos[turn][i], s_sin[turn][i]);
+          __syncthreads();
+          const int i = (HALF ? l & (LPH / 2 - 1) : l) * 4;
+          c = pairs(*reinterpret_cast<const float4*>(&s_cos[turn][i]));
+          s = pairs(*reinterpret_cast<const float4*>(&s_sin[turn][i]));
+          ns = mul(s, all(-1.0f));
+          if (HALF && l < LPH / 2) s = ns;  // what turns with the partner: -sin in the first half, sin in the second
+          if (next) entry_next = m.table_off[seq_next] + p_next / bs;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * step;
+          if (h - sub >= total) break;  // no head of this warp
+          const bool is_q = h < heads, is_v = h >= heads + kv_heads;
+          Pair2 y0 = pairs(x[u][0]), y1 = pairs(x[u][1]);
+          if (bias && h < total) {
+            y0 = add(y0, pairs(*reinterpret_cast<const float4*>(bias + h * D + l * 4)));
+            y1 = add(y1, pairs(*reinterpret_cast<const float4*>(bias + h * D + D / 2 + l * 4)));
+          }
+          const float* w = is_q ? q_norm : (is_v ? nullptr : k_norm);
+          if (HPW > 1 ? (q_norm || k_norm) : w != nullptr) {
+            const Pair2 sq = fma(y1, y1, mul(y0, y0));
+            float ss = (sq.a.x + sq.a.y) + (sq.b.x + sq.b.y);
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (w) {
+              const Pair2 scale = all(rsqrtf(ss * (1.0f / D) + eps));
+              y0 = mul(y0, mul(scale, pairs(reinterpret_cast<const float4*>(w)[l])));
+              y1 = mul(y1, mul(scale, pairs(reinterpret_cast<const float4*>(w)[l + LPH])));
+            }
+          }
+          if constexpr (HALF) {
+            Pair2 z;
+            z.a.x = __shfl_xor_sync(0xffffffffu, y0.a.x, LPH / 2), z.a.y = __shfl_xor_sync(0xffffffffu, y0.a.y, LPH / 2);
+            z.b.x = __shfl_xor_sync(0xffffffffu, y0.b.x, LPH / 2), z.b.y = __shfl_xor_sync(0xffffffffu, y0.b.y, LPH / 2);
+            if (!is_v) y0 = fma(z, s, mul(y0, c));
+          } else if (!is_v) {
+            const Pair2 z = y0;
+            y0 = fma(y1, ns, mul(y0, c));
+            y1 = fma(z, s, mul(y1, c));
+          }
+          if (h >= total) continue;
+          if (is_q) {
+            *reinterpret_cast<float4*>(dst + h * D) = make_float4(y0.a.x, y0.a.y, y0.b.x, y0.b.y);
+            *reinterpret_cast<float4*>(dst + h * D + D / 2) = make_float4(y1.a.x, y1.a.y, y1.b.x, y1.b.y);
+          } else {
+            __half* to = (is_v ? vc : kc) + page + (is_v ? h - heads - kv_heads : h - heads) * bs * D;
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack_half2(y0.a.x, y0.a.y), pack_half2(y0.b.x, y0.b.y));
+            *reinterpret_cast<uint2*>(to + D / 2) = make_uint2(pack_half2(y1.a.x, y1.a.y), pack_half2(y1.b.x, y1.b.y));
+          }
+        }
+      }
+      turn ^= 1;
+    }
+    if (t_next >= T) break;
+    if (next && entry_next < 0) entry_next = m.table_off[seq_next] + p_next / bs;  // this token was padding
+    block = next ? m.tables[entry_next] : 0;
+    t = t_next, seq = seq_next, p = p_next;
+  }
+}
+
 // One CTA per token. A head is held by LPH lanes, lane l with the vectors (4 values) l and, with NV = 2,
 // l + LPH; a warp takes 32 / LPH heads at a time and has U such rounds in flight, so that a token's
 // whole row is under way before anything waits. The rotation angles and the page lookup (three
 // dependent loads) run under those loads. The partner of a rotated vector is rot/8 vectors away, in
 // another lane: it comes by shuffle.
-// FULL: every lane holds values (head_dim = 4 LPH NV) and the whole head is rotated.
-template <int LPH, int NV, bool FULL>
+template <int LPH, int NV>
 __global__ void __launch_bounds__(512, 2)
 qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const float* __restrict__ q_norm,
                     const float* __restrict__ k_norm, float eps, const float* __restrict__ inv_freq, int rot, TokenMeta m,
                     float* q_out, __half* __restrict__ kc, __half* __restrict__ vc, int heads, int kv_heads, int D, int bs,
                     int qkv_stride, int q_stride) {
   constexpr int HPW = 32 / LPH, U = kQnRounds / NV;
-  if constexpr (FULL) D = rot = 4 * LPH * NV;
   extern __shared__ float sm[];  // [rot/2] cos, [rot/2] -sin, [rot/2] sin
   pdl_trigger();
   pdl_wait();
@@ -61,7 +173,7 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
       const int h = h0 + u * step;
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-        x[u][n] = h < total && (FULL || l + n * LPH < vecs) ? *reinterpret_cast<const float4*>(src + h * D + n * LPH * 4)
+        x[u][n] = h < total && l + n * LPH < vecs ? *reinterpret_cast<const float4*>(src + h * D + n * LPH * 4)
                                                             : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (h0 < step) {  // the first time round, which every warp makes
@@ -80,7 +192,7 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
       for (int n = 0; n < NV; ++n) {
         const int v = l + n * LPH;
         cs[n] = make_float4(1.f, 1.f, 1.f, 1.f), sn[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (FULL || v < 2 * h4) {
+        if (v < 2 * h4) {
           const int i = (v < h4 ? v : v - h4) * 4;
           cs[n] = *reinterpret_cast<const float4*>(sm + i);
           sn[n] = *reinterpret_cast<const float4*>(sm + (v < h4 ? half : 2 * half) + i);
@@ -95,7 +207,7 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
       if (bias && there) {
 #pragma unroll
         for (int n = 0; n < NV; ++n)
-          if (FULL || l + n * LPH < vecs) {
+          if (l + n * LPH < vecs) {
             const float4 b = *reinterpret_cast<const float4*>(bias + h * D + (l + n * LPH) * 4);
             x[u][n].x += b.x, x[u][n].y += b.y, x[u][n].z += b.z, x[u][n].w += b.w;
           }
@@ -113,7 +225,7 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
             const float scale = rsqrtf(ss * inv_d + eps);
 #pragma unroll
             for (int n = 0; n < NV; ++n)
-              if (FULL || l + n * LPH < vecs) {
+              if (l + n * LPH < vecs) {
                 const float4 g = reinterpret_cast<const float4*>(w)[l + n * LPH];
                 x[u][n].x *= scale * g.x, x[u][n].y *= scale * g.y, x[u][n].z *= scale * g.z, x[u][n].w *= scale * g.w;
               }
@@ -123,24 +235,20 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
           // the partner of vector v: v + h4 for the first h4 vectors, v - h4 for the next h4
-          if constexpr (FULL && NV == 2) {
-            z[n] = x[u][1 - n];
-          } else {
-            const int v = l + n * LPH, pv = v < h4 ? v + h4 : v - h4;
-            const int from = FULL ? lane ^ (LPH / 2) : sub * LPH + (pv & (LPH - 1));
-            z[n].x = __shfl_sync(0xffffffffu, x[u][0].x, from), z[n].y = __shfl_sync(0xffffffffu, x[u][0].y, from);
-            z[n].z = __shfl_sync(0xffffffffu, x[u][0].z, from), z[n].w = __shfl_sync(0xffffffffu, x[u][0].w, from);
-            if constexpr (NV == 2) {
-              const float4 z1 = make_float4(__shfl_sync(0xffffffffu, x[u][1].x, from), __shfl_sync(0xffffffffu, x[u][1].y, from),
-                                            __shfl_sync(0xffffffffu, x[u][1].z, from), __shfl_sync(0xffffffffu, x[u][1].w, from));
-              if (pv >= LPH) z[n] = z1;
-            }
+          const int v = l + n * LPH, pv = v < h4 ? v + h4 : v - h4;
+          const int from = sub * LPH + (pv & (LPH - 1));
+          z[n].x = __shfl_sync(0xffffffffu, x[u][0].x, from), z[n].y = __shfl_sync(0xffffffffu, x[u][0].y, from);
+          z[n].z = __shfl_sync(0xffffffffu, x[u][0].z, from), z[n].w = __shfl_sync(0xffffffffu, x[u][0].w, from);
+          if constexpr (NV == 2) {
+            const float4 z1 = make_float4(__shfl_sync(0xffffffffu, x[u][1].x, from), __shfl_sync(0xffffffffu, x[u][1].y, from),
+                                          __shfl_sync(0xffffffffu, x[u][1].z, from), __shfl_sync(0xffffffffu, x[u][1].w, from));
+            if (pv >= LPH) z[n] = z1;
           }
         }
         if (!is_v) {
 #pragma unroll
           for (int n = 0; n < NV; ++n) {
-            if (!FULL && l + n * LPH >= 2 * h4) continue;  // passes: its "partner" may hold anything
+            if (l + n * LPH >= 2 * h4) continue;  // passes: its "partner" may hold anything
             x[u][n].x = x[u][n].x * cs[n].x + z[n].x * sn[n].x, x[u][n].y = x[u][n].y * cs[n].y + z[n].y * sn[n].y;
             x[u][n].z = x[u][n].z * cs[n].z + z[n].z * sn[n].z, x[u][n].w = x[u][n].w * cs[n].w + z[n].w * sn[n].w;
           }
@@ -149,7 +257,7 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
       if (!there) continue;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        if (!FULL && l + n * LPH >= vecs) continue;
+        if (l + n * LPH >= vecs) continue;
         if (is_q) {
           *reinterpret_cast<float4*>(dst + h * D + n * LPH * 4) = x[u][n];
         } else {
@@ -223,19 +331,34 @@ void launch_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, c
   auto aligned = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   if (D % 4 == 0 && rot % 8 == 0 && qkv_stride % 4 == 0 && q_stride % 4 == 0 && aligned(qkv, 16) && aligned(q_out, 16) &&
       aligned(bias, 16) && aligned(q_norm, 16) && aligned(k_norm, 16) && aligned(kc, 8) && aligned(vc, 8)) {
+    // A few tokens: as many warps as have the whole row in flight, the shortest way through. Many: fewer, with the
+    // rounds even among them, so that more tokens are under way on an SM. At 32 + 2 x 8 heads of 128, 8 x 2048
+    // tokens take 113 us with six warps, 118 with eight, 126 with four.
+    const bool many = T > 2 * sm_count();
+    auto warps_for = [&](int per_warp, int in_flight, int most) {
+      const int turns = div_up(heads + 2 * kv_heads, per_warp * in_flight);  // of one warp, for the whole row
+      return many ? div_up(turns, div_up(turns, most)) : std::min(16, turns);
+    };
+    if ((D == 32 || D == 64 || D == 128 || D == 256) && (rot == D || rot == D / 2)) {
+      const bool half = rot != D;
+      auto kernel = D == 256   ? (half ? qkv_norm_pair_kernel<32, true> : qkv_norm_pair_kernel<32, false>)
+                    : D == 128 ? (half ? qkv_norm_pair_kernel<16, true> : qkv_norm_pair_kernel<16, false>)
+                    : D == 64  ? (half ? qkv_norm_pair_kernel<8, true> : qkv_norm_pair_kernel<8, false>)
+                               : (half ? qkv_norm_pair_kernel<4, true> : qkv_norm_pair_kernel<4, false>);
+      const int warps = warps_for(256 / D, kQnPairRounds, 6);
+      const int ctas = many ? std::min(T, sm_count() * (1024 / (warps * 32))) : T;  // what 64 registers a thread let an SM hold
+      launch_pdl(kernel, dim3(ctas), dim3(warps * 32), 0, st, qkv, bias, q_norm, k_norm, eps, inv_freq, m, T, q_out, kc, vc, heads, kv_heads,
+                 block_size, qkv_stride, q_stride);
+      return;
+    }
     const int lanes = D > 64 ? 32 : (D > 32 ? 16 : 8), nv = D > 128 ? 2 : 1;
-    // A few tokens: a warp for every kQnRounds rounds, the shortest way through. Many: at most eight warps, so that
-    // more tokens are under way on an SM (8 x 2048 tokens at 32 + 2 x 8 heads of 128: 139 us with 8 warps, 169
-    // with 12; 256 tokens: 4.9 and 3.6 us).
-    const int rounds = div_up(heads + 2 * kv_heads, 32 / lanes);
-    const int warps = T > 2 * sm_count() ? std::min(8, rounds) : std::min(16, div_up(rounds, kQnRounds / nv));
-    const bool full = rot == D && D == 4 * lanes * nv;
-    auto kernel = nv == 2       ? (full ? qkv_norm_vec_kernel<32, 2, true> : qkv_norm_vec_kernel<32, 2, false>)
-                  : lanes == 32 ? (full ? qkv_norm_vec_kernel<32, 1, true> : qkv_norm_vec_kernel<32, 1, false>)
-                  : lanes == 16 ? (full ? qkv_norm_vec_kernel<16, 1, true> : qkv_norm_vec_kernel<16, 1, false>)
-                                : (full ? qkv_norm_vec_kernel<8, 1, true> : qkv_norm_vec_kernel<8, 1, false>);
-    launch_pdl(kernel, dim3(T), dim3(warps * 32), rot / 2 * 3 * sizeof(float), st, qkv, bias, q_norm, k_norm, eps, inv_freq, rot, m, q_out, kc, vc,
-               heads, kv_heads, D, block_size, qkv_stride, q_stride);
+    const int warps = warps_for(32 / lanes, kQnRounds / nv, 8);
+    auto kernel = nv == 2       ? qkv_norm_vec_kernel<32, 2>
+                  : lanes == 32 ? qkv_norm_vec_kernel<32, 1>
+                  : lanes == 16 ? qkv_norm_vec_kernel<16, 1>
+                                : qkv_norm_vec_kernel<8, 1>;
+    launch_pdl(kernel, dim3(T), dim3(warps * 32), rot / 2 * 3 * sizeof(float), st, qkv, bias, q_norm, k_norm, eps, inv_freq, rot, m, q_out, kc,
+               vc, heads, kv_heads, D, block_size, qkv_stride, q_stride);
     return;
   }
   const size_t smem = (static_cast<size_t>(rot) + kQnWarps * D) * sizeof(float);
