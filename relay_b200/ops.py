@@ -93,34 +93,46 @@ def decode_attention_static(shape: CAttnShape, q, meta: TokenMeta, decode_tokens
 
 def _here(op: str, name: str, t: torch.Tensor) -> int:
     """The current CUDA device, which an operator's tensors have to be on; `t` is the first of them."""
-    if not t.is_cuda:
+    here = t.get_device()
+    if here < 0 or here != torch.cuda.current_device():
         raise ValueError(f"{op}: {name} must be on the current CUDA device, not on {t.device}")
-    return torch.cuda.current_device()
+    return here
 
 
-def _check_tensors(op: str, here: int, *named) -> None:
-    """Each (name, tensor, dtype) has that type and contiguous rows and lies on device `here`; None passes."""
-    for name, t, dtype in named:
+def _plain(here: int, dtype: torch.dtype, *tensors) -> bool:
+    """Whether each tensor has that type, is contiguous and lies on device `here`; None passes."""
+    for t in tensors:
+        if t is not None and (t.dtype is not dtype or t.get_device() != here or not t.is_contiguous()):
+            return False
+    return True
+
+
+def _complain(op: str, here: int, *named) -> None:
+    """Says what is wrong with the first (name, tensor, dtype, whole) that is not of that type on device `here`, with
+    contiguous rows or, where `whole`, contiguous altogether."""
+    for name, t, dtype, whole in named:
         if t is None:
             continue
         if t.dtype is not dtype:
             raise ValueError(f"{op}: {name} must be {dtype}, not {t.dtype}")
         if t.get_device() != here:
             raise ValueError(f"{op}: {name} must be on the current CUDA device {here}, not on {t.device}")
-        if not t.is_contiguous() and t.size(-1) > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{op}: the rows of {name} must be contiguous")
+        if not t.is_contiguous() and (whole or t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1)):
+            raise ValueError(f"{op}: {name} must be contiguous" if whole else f"{op}: the rows of {name} must be contiguous")
 
 
 def _check_meta(op: str, here: int, meta: TokenMeta, tokens: int) -> None:
-    _check_tensors(op, here, ("pos", meta.pos, torch.int32), ("seq", meta.seq, torch.int32),
-                   ("table_off", meta.table_off, torch.int32), ("tables", meta.tables, torch.int32))
+    if not _plain(here, torch.int32, meta.pos, meta.seq, meta.table_off, meta.tables):
+        _complain(op, here, *((name, getattr(meta, name), torch.int32, True) for name in ("pos", "seq", "table_off", "tables")))
     if meta.pos.numel() < tokens or meta.seq.numel() < tokens:
         raise ValueError(f"{op}: the metadata must have an entry for each token")
 
 
-def _check_pools(op: str, page, k_pool, v_pool) -> None:
-    if k_pool.shape[1:] != page or v_pool.shape[1:] != page or not k_pool.is_contiguous() or not v_pool.is_contiguous():
-        raise ValueError(f"{op}: the pools must be contiguous [blocks, kv_heads, block_size, head_dim] tensors")
+def _check_pools(op: str, here: int, page, k_pool, v_pool) -> None:
+    if not _plain(here, torch.float16, k_pool, v_pool):
+        _complain(op, here, ("k_pool", k_pool, torch.float16, True), ("v_pool", v_pool, torch.float16, True))
+    if k_pool.shape[1:] != page or v_pool.shape[1:] != page:
+        raise ValueError(f"{op}: the pools must be [blocks, kv_heads, block_size, head_dim] tensors")
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -143,19 +155,23 @@ def shared_prefix_attention(shape: CAttnShape, q: torch.Tensor, meta: TokenMeta,
     group_off[g] .. group_off[g + 1] - 1 of decode_tokens share their first prefix_len[g] keys, which
     are read once for the group. max_prefix / max_suffix (the longest shared part, the most keys
     behind it) only decide how the work is split. A step captured as a graph passes its own scratch."""
-    op, i32, f16 = "shared_prefix_attention", torch.int32, torch.float16
-    n, n_groups, rows, here = decode_tokens.numel(), prefix_len.numel(), meta.pos.numel(), _here("shared_prefix_attention", "q", q)
-    _check_tensors(op, here, ("q", q, torch.float32), ("decode_tokens", decode_tokens, i32), ("group_off", group_off, i32),
-                   ("prefix_len", prefix_len, i32), ("k_pool", k_pool, f16), ("v_pool", v_pool, f16), ("out", out, f16),
-                   ("scratch", scratch, torch.uint8))
+    op = "shared_prefix_attention"
+    here, n, n_groups, rows = _here(op, "q", q), decode_tokens.numel(), prefix_len.numel(), meta.pos.numel()
+    if not (_plain(here, torch.int32, decode_tokens, group_off, prefix_len) and _plain(here, torch.float32, q) and
+            _plain(here, torch.float16, out) and _plain(here, torch.uint8, scratch)):
+        i32 = torch.int32
+        _complain(op, here, ("decode_tokens", decode_tokens, i32, True), ("group_off", group_off, i32, True),
+                  ("prefix_len", prefix_len, i32, True), ("q", q, torch.float32, False), ("out", out, torch.float16, False),
+                  ("scratch", scratch, torch.uint8, True))
     _check_meta(op, here, meta, rows)
-    _check_pools(op, (shape.kv_heads, shape.block_size, shape.head_dim), k_pool, v_pool)
+    _check_pools(op, here, (shape.kv_heads, shape.block_size, shape.head_dim), k_pool, v_pool)
     if group_off.numel() != n_groups + 1:
         raise ValueError(f"{op}: group_off must have one entry more than prefix_len")
     width = shape.heads * shape.head_dim
-    for name, t, stride in (("q", q, shape.q_stride), ("out", out, shape.o_stride)):
-        if t.dim() != 2 or t.size(0) < rows or t.size(1) < width or (rows > 1 and t.stride(0) != stride):
-            raise ValueError(f"{op}: {name} must have the batch's rows, {stride} values apart")
+    if q.dim() != 2 or q.size(0) < rows or q.size(1) < width or (rows > 1 and q.stride(0) != shape.q_stride):
+        raise ValueError(f"{op}: q must have the batch's rows, {shape.q_stride} values apart")
+    if out.dim() != 2 or out.size(0) < rows or out.size(1) < width or (rows > 1 and out.stride(0) != shape.o_stride):
+        raise ValueError(f"{op}: out must have the batch's rows, {shape.o_stride} values apart")
     L, sh, m = _lib.lib(), C.byref(shape), meta.c()
     if scratch is None:
         scratch = torch.empty(max(L.rb200_shared_prefix_scratch_bytes(sh, n, n_groups, max_prefix, max_suffix), 16), dtype=torch.uint8,
@@ -239,10 +255,11 @@ def qkv_norm_post(qkv, bias, q_norm, k_norm, eps, inv_freq, meta: TokenMeta, q_o
     """qkv_post with an RMS norm over each query and key head (q_norm, k_norm [head_dim], or None) ahead of
     the rotation of its first rot_dim values (default: all): q to q_out (which may be qkv), k and v to
     their pages. A token with seq or pos below 0 is padding."""
-    op, f32, f16 = "qkv_norm_post", torch.float32, torch.float16
-    rot, here = head_dim if rot_dim is None else rot_dim, _here("qkv_norm_post", "qkv", qkv)
-    _check_tensors(op, here, ("qkv", qkv, f32), ("bias", bias, f32), ("q_norm", q_norm, f32), ("k_norm", k_norm, f32),
-                   ("inv_freq", inv_freq, f32), ("q_out", q_out, f32), ("k_pool", k_pool, f16), ("v_pool", v_pool, f16))
+    op, f32, rot = "qkv_norm_post", torch.float32, head_dim if rot_dim is None else rot_dim
+    here = _here(op, "qkv", qkv)
+    if not _plain(here, f32, qkv, bias, q_norm, k_norm, inv_freq, q_out):
+        _complain(op, here, ("qkv", qkv, f32, False), ("bias", bias, f32, True), ("q_norm", q_norm, f32, True),
+                  ("k_norm", k_norm, f32, True), ("inv_freq", inv_freq, f32, True), ("q_out", q_out, f32, False))
     width = (heads + 2 * kv_heads) * head_dim
     if qkv.dim() != 2 or qkv.size(1) < width:
         raise ValueError(f"{op}: qkv must be [tokens, (heads + 2 kv_heads) head_dim]")
@@ -250,10 +267,13 @@ def qkv_norm_post(qkv, bias, q_norm, k_norm, eps, inv_freq, meta: TokenMeta, q_o
     if q_out.dim() != 2 or q_out.size(0) < T or q_out.size(1) < heads * head_dim:
         raise ValueError(f"{op}: q_out must be [tokens, heads head_dim]")
     _check_meta(op, here, meta, T)
-    _check_pools(op, (kv_heads, block_size, head_dim), k_pool, v_pool)
-    for name, t, n in (("bias", bias, width), ("q_norm", q_norm, head_dim), ("k_norm", k_norm, head_dim), ("inv_freq", inv_freq, rot // 2)):
-        if t is not None and t.numel() != n:
-            raise ValueError(f"{op}: {name} must have {n} values")
+    _check_pools(op, here, (kv_heads, block_size, head_dim), k_pool, v_pool)
+    if bias is not None and bias.numel() != width:
+        raise ValueError(f"{op}: bias must have {width} values")
+    if (q_norm is not None and q_norm.numel() != head_dim) or (k_norm is not None and k_norm.numel() != head_dim):
+        raise ValueError(f"{op}: q_norm and k_norm must have {head_dim} values")
+    if inv_freq is not None and inv_freq.numel() != rot // 2:
+        raise ValueError(f"{op}: inv_freq must have {rot // 2} values")
     m = meta.c()
     _lib.check(_lib.lib().rb200_qkv_norm_post(
         qkv.data_ptr(), _row_stride(qkv), _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), rot, C.byref(m), T,
@@ -297,28 +317,32 @@ def adjust_logits(logits, out, penalties=None, history=None, history_len=None, p
     of history [R][.], of which the first prompt_len are the prompt; bias_values for the first bias_len
     of bias_ids [R][.], the last entry of a token counting; and a mask [R][ceil(V / 32)] of int32 words,
     whose 0 bits become -inf. Ids outside the vocabulary are passed over."""
-    op, f32, i32, here = "adjust_logits", torch.float32, torch.int32, _here("adjust_logits", "logits", logits)
-    _check_tensors(op, here, ("logits", logits, f32), ("out", out, f32), ("penalties", penalties, f32), ("history", history, i32),
-                   ("history_len", history_len, i32), ("prompt_len", prompt_len, i32), ("bias_ids", bias_ids, i32),
-                   ("bias_values", bias_values, f32), ("bias_len", bias_len, i32), ("mask", mask, i32))
+    op, f32, i32 = "adjust_logits", torch.float32, torch.int32
+    here = _here(op, "logits", logits)
+    if not (_plain(here, f32, logits, out, penalties, bias_values) and
+            _plain(here, i32, history, history_len, prompt_len, bias_ids, bias_len, mask)):
+        _complain(op, here, ("logits", logits, f32, False), ("out", out, f32, False), ("penalties", penalties, f32, True),
+                  ("history", history, i32, True), ("history_len", history_len, i32, True), ("prompt_len", prompt_len, i32, True),
+                  ("bias_ids", bias_ids, i32, True), ("bias_values", bias_values, f32, True), ("bias_len", bias_len, i32, True),
+                  ("mask", mask, i32, False))
     if logits.dim() != 2 or out.shape != logits.shape:
         raise ValueError(f"{op}: logits and out must both be [rows, vocabulary]")
     R, V = logits.shape
-    for name, t in (("history_len", history_len), ("prompt_len", prompt_len), ("bias_len", bias_len)):
-        if t is not None and (t.numel() != R or not t.is_contiguous()):
-            raise ValueError(f"{op}: {name} must have an entry for each row")
-    for name, t in (("penalties", penalties), ("history", history), ("bias_ids", bias_ids), ("bias_values", bias_values)):
-        if t is not None and (t.dim() != 2 or t.size(0) != R or not t.is_contiguous()):
-            raise ValueError(f"{op}: {name} must be a contiguous tensor with the rows of logits")
-    if penalties is not None and (penalties.size(1) != 4 or history is None or history_len is None):
-        raise ValueError(f"{op}: penalties must be [rows, 4] and need a history")
-    if bias_ids is not None and (bias_values is None or bias_len is None or bias_ids.shape != bias_values.shape):
-        raise ValueError(f"{op}: bias_ids need values of the same shape and lengths")
+    if penalties is not None:
+        if history is None or history_len is None or penalties.shape != (R, 4):
+            raise ValueError(f"{op}: penalties must be [rows, 4] and need a history")
+        if history.dim() != 2 or history.size(0) != R or history_len.numel() != R or (prompt_len is not None and prompt_len.numel() != R):
+            raise ValueError(f"{op}: history must be [rows, tokens] with a length, and a prompt length, for each row")
+    if bias_ids is not None:
+        if bias_values is None or bias_len is None or bias_ids.shape != bias_values.shape:
+            raise ValueError(f"{op}: bias_ids need values of the same shape and lengths")
+        if bias_ids.dim() != 2 or bias_ids.size(0) != R or bias_len.numel() != R:
+            raise ValueError(f"{op}: bias_ids must be [rows, entries] with a length for each row")
     if mask is not None and (mask.dim() != 2 or mask.size(0) != R or mask.size(1) * 32 < V):
         raise ValueError(f"{op}: mask must be [rows, ceil(vocabulary / 32)]")
     _lib.check(_lib.lib().rb200_adjust_logits(
         logits.data_ptr(), _row_stride(logits), out.data_ptr(), _row_stride(out), R, V, _ptr(penalties), _ptr(history),
-        0 if history is None else history.size(1), _ptr(history_len), _ptr(prompt_len), _ptr(bias_ids), _ptr(bias_values),
+        0 if penalties is None else history.size(1), _ptr(history_len), _ptr(prompt_len), _ptr(bias_ids), _ptr(bias_values),
         0 if bias_ids is None else bias_ids.size(1), _ptr(bias_len), _ptr(mask), 0 if mask is None else _row_stride(mask),
         _raw_stream(here)))
     return out
