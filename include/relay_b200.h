@@ -391,7 +391,8 @@ int rb200_decode_attention_static(const rb200_attn_shape* s, const float* q, con
  *  - A group counts min(prefix_len[g], context of its first entry) keys as shared; 0 is allowed,
  *    and so is any length, also one that ends inside a block (the blocks up to there have to hold
  *    the same keys, they need not be the same blocks). An entry with a shorter context than its
- *    group's prefix sees its own context only.
+ *    group's prefix sees its own context only; the shared keys behind it get the weight 0, so
+ *    their V has to be finite. A batch row that two entries name gets the result of either.
  *  - An entry of decode_tokens below 0, and every entry before group_off[0] or from
  *    group_off[n_groups] on, is padding: its row of out is left as it was. An entry without keys
  *    (pos < 0) gets zeros.
@@ -400,8 +401,11 @@ int rb200_decode_attention_static(const rb200_attn_shape* s, const float* q, con
  *    rounding. max_prefix 0: nothing is read as shared.
  *  - scratch (rb200_shared_prefix_scratch_bytes, 16-byte aligned, no initial state) holds the
  *    partial results of this call: calls that may overlap need one each.
- * head_dim 16, 32, 64 or 128, at most 16 query heads per KV head; q 16-byte aligned with
- * q_stride a multiple of 4, the pools and out 16-byte aligned with o_stride a multiple of 8. */
+ *  - The first call on a device allocates a status word (rb200_gemm_status): make it outside stream
+ *    capture.
+ * head_dim 16, 32, 64 or 128, at most 16 query heads per KV head; q finite in fp16 (up to 65504) and
+ * 16-byte aligned with q_stride a multiple of 4, the pools and out 16-byte aligned with o_stride a
+ * multiple of 8. */
 size_t rb200_shared_prefix_scratch_bytes(const rb200_attn_shape* s, int n_decode, int n_groups, int max_prefix,
                                          int max_suffix);
 int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, const rb200_token_meta* m,
@@ -449,8 +453,9 @@ int rb200_gemv_f16(const void* w, const void* x, float* y, int T, int K, int N, 
 int rb200_gemm(const void* w_f16, const int8_t* w_i8, const float* scale, const void* x, float* y, int T, int K,
                int N, int ldw, int ldx, float beta, void* stream);
 
-/* 0, or the code that a bounded pipeline wait inside the tensor-core GEMM left on the
- * current device when it gave up (the launch then produced no valid output). */
+/* 0, or the code that a bounded pipeline wait inside a tensor-core kernel (GEMM, prefill attention,
+ * shared-prefix attention) left on the current device when it gave up (the launch then produced no
+ * valid output). */
 int rb200_gemm_status(void);
 
 /* rmsnorm_kernel (engine/src/cuda_backend.cu:157-167): out[r] = w * x[rows ? rows[r] : r] * rsqrt(mean(x^2)+eps),
@@ -505,7 +510,7 @@ int rb200_argmax_rows(const float* logits, int R, int V, int32_t* token_out, flo
  * Ids outside [0, V) (padding) are passed over, as are bits behind V; a length above its leading
  * dimension counts as that, one below 0 as 0. logits and out rows are ld_logits and ld_out
  * floats apart; out may be logits itself with the same stride, any other overlap is not allowed.
- * Columns from V on are left as they were. */
+ * Columns from V on are left as they were. R is at most 65535. */
 typedef struct rb200_penalties {
   float repetition; /* > 0; 1: none */
   float presence;   /* 0: none */

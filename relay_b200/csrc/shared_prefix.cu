@@ -656,6 +656,7 @@ int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, con
     RB_REQUIRE(fast_attention_supported(sh), "shared prefix attention: head_dim must be 16/32/64/128 and heads/kv_heads <= 16");
     RB_REQUIRE(sh.q_stride % 4 == 0 && sh.o_stride % 8 == 0, "shared prefix attention: q_stride must be a multiple of 4, o_stride of 8");
     RB_REQUIRE(n_decode >= 0 && n_groups >= 0 && max_prefix >= 0 && max_suffix >= 0, "shared prefix attention: bad batch");
+    RB_REQUIRE(static_cast<long long>(n_decode) * sh.heads <= 0x7fffffff, "shared prefix attention: bad batch (too many entries)");
     if (n_decode == 0 || n_groups == 0) return 0;  // every entry is padding
     RB_REQUIRE(q && m && m->pos && m->seq && m->table_off && m->tables && decode_tokens && group_off && prefix_len && k_pool &&
                    v_pool && scratch && out,

@@ -125,6 +125,58 @@ def test_qkv_norm_post(ops, D, heads, kv_heads, bs, rot, use_bias, norms, chunks
     assert np.all(gk[rest] == 9) and np.all(gv[rest] == 9)  # no other slot is touched
 
 
+@pytest.mark.parametrize("D,rot", [(128, 128), (64, 32), (80, 80)])
+@pytest.mark.parametrize("shift,pad", [(1, 3), (2, 0), (0, 1)])
+def test_qkv_norm_post_of_unaligned_rows(ops, D, rot, shift, pad):
+    # rows that start anywhere in memory: the same values as from aligned ones, up to the order of a head's sum
+    rng = np.random.Generator(np.random.PCG64(D + shift))
+    heads, kv_heads, bs, T = 6, 2, 16, 21
+    width = (heads + 2 * kv_heads) * D
+    flat = torch.zeros(shift + T * (width + pad), device="cuda")
+    qkv = flat[shift:].view(T, width + pad)
+    qkv[:, :width] = dev(rng.standard_normal((T, width)).astype(np.float32))
+    qn, kn = (dev((1 + 0.1 * rng.standard_normal(D)).astype(np.float32)) for _ in range(2))
+    inv = (10000.0 ** -(np.arange(0, rot, 2) / rot)).astype(np.float32)
+    meta = ops.TokenMeta.from_host(np.arange(T) + 5, np.zeros(T), [0], [1, 0])
+    kp = torch.zeros((2, kv_heads, bs, D), dtype=torch.float16, device="cuda")
+    vp = torch.zeros_like(kp)
+    q_out = torch.zeros((T, heads * D + 1), device="cuda")
+    ops.qkv_norm_post(qkv, None, qn, kn, 1e-6, dev(inv), meta, q_out, kp, vp, heads, kv_heads, D, bs, rot_dim=rot)
+    q, k, v, reach = norm_rope_f64(qkv[:, :width].cpu().numpy(), None, qn.cpu().numpy(), kn.cpu().numpy(), 1e-6, inv,
+                                   np.arange(T) + 5, heads, kv_heads, D, rot)
+    got = q_out.cpu().numpy()
+    assert np.all(np.abs(got[:, :heads * D].reshape(q.shape) - q) <= NORM_TOL * reach[:, :heads])
+    assert np.all(got[:, heads * D:] == 0)
+    gv = vp.cpu().numpy()
+    for t in range(T):
+        assert np.array_equal(gv[[1, 0][(t + 5) // bs], :, (t + 5) % bs], v[t].astype(np.float16))
+
+
+def test_qkv_norm_post_of_more_tokens_than_the_grid_holds(ops):
+    # many tokens, padding among them: a CTA goes through several
+    rng = np.random.Generator(np.random.PCG64(11))
+    heads, kv_heads, D, bs, T = 4, 1, 64, 16, 6001
+    width = (heads + 2 * kv_heads) * D
+    qkv = rng.standard_normal((T, width)).astype(np.float32)
+    pos, seq = np.arange(T, dtype=np.int32), np.zeros(T, np.int32)
+    pad = rng.random(T) < 0.1
+    pad[[0, T - 1]] = True
+    seq[pad] = -1
+    inv = (10000.0 ** -(np.arange(0, D, 2) / D)).astype(np.float32)
+    nb = (T + bs - 1) // bs
+    table = rng.permutation(nb).astype(np.int32)
+    meta = ops.TokenMeta.from_host(pos, seq, [0], table)
+    kp = torch.full((nb, kv_heads, bs, D), 9.0, dtype=torch.float16, device="cuda")
+    vp = kp.clone()
+    q_out = torch.full((T, heads * D), 5.0, device="cuda")
+    ops.qkv_norm_post(dev(qkv), None, None, None, 1e-6, dev(inv), meta, q_out, kp, vp, heads, kv_heads, D, bs)
+    q, k, v, reach = norm_rope_f64(qkv, None, None, None, 1e-6, inv, pos, heads, kv_heads, D, D)
+    got = q_out.cpu().numpy().reshape(q.shape)
+    assert np.all(got[pad] == 5) and np.all(np.abs(got - q)[~pad] <= NORM_TOL * reach[:, :heads][~pad])
+    rows = vp[torch.from_numpy(table).long()].transpose(1, 2).reshape(nb * bs, kv_heads, D)[:T].cpu().numpy()
+    assert np.all(rows[pad] == 9) and np.array_equal(rows[~pad], v[~pad].astype(np.float16))
+
+
 def test_qkv_norm_post_without_norms_agrees_with_qkv_post(ops):
     rng = np.random.Generator(np.random.PCG64(5))
     heads, kv_heads, D, bs, T = 8, 2, 64, 16, 40
@@ -313,6 +365,24 @@ def test_shared_prefix_attention_agrees_with_decode_attention(ops, D, heads, kv_
     want = out.cpu().numpy().astype(np.float32)[c["tokens"]]
     # two kernels, each within the bound of check_prefix
     assert np.abs(got[c["tokens"]] - want).max() <= 4 * (H16 + 2.0 ** -15) * np.abs(c["v"][~np.isnan(c["v"])].astype(np.float32)).max()
+
+
+@pytest.mark.parametrize("D,bs", [(128, 16), (32, 8)])
+def test_shared_prefix_attention_of_a_padded_batch(ops, D, bs):
+    # entries before the first group and behind the last are padding, whatever they name
+    c = prefix_case(12, D, 8, 2, bs, [(300, [5, 40]), (17, [1, 2, 3])])
+    c["tokens"] = np.concatenate([[c["tokens"][1], -1], c["tokens"], [c["tokens"][0]] * 3]).astype(np.int32)
+    c["off"] = c["off"] + 2
+    out = run_prefix(ops, c)
+    c["tokens"], c["off"] = c["tokens"][2:-3], c["off"] - 2
+    check_prefix(c, out, 7.0)
+
+
+def test_shared_prefix_attention_of_the_same_row_twice(ops):
+    c = prefix_case(13, 64, 8, 2, 16, [(300, [5, 40, 7])])
+    want = run_prefix(ops, c)
+    c["tokens"], c["off"] = np.concatenate([c["tokens"], c["tokens"][:1]]), np.asarray([0, 4], np.int32)
+    assert np.array_equal(run_prefix(ops, c), want)  # one group: either result has the same bits
 
 
 def test_shared_prefix_attention_scratch_may_hold_anything(ops):

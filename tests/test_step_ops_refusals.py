@@ -59,7 +59,7 @@ def prefix(shape=(32, 8, 128, 16, 6144, 4096), **kw):
     (dict(shape=(34, 2, 64, 16, 4096, 4096)), "heads/kv_heads"),
     (dict(shape=(32, 8, 128, 16, 4095, 4096)), "strides too small"), (dict(shape=(32, 8, 128, 16, 6144, 4095)), "strides too small"),
     (dict(shape=(32, 8, 128, 16, 6146, 4096)), "multiple"), (dict(shape=(32, 8, 128, 16, 6144, 4100)), "multiple"),
-    (dict(n=-1), "bad batch"), (dict(groups=-1), "bad batch"), (dict(max_prefix=-1), "bad batch"), (dict(max_suffix=-1), "bad batch"),
+    (dict(n=-1), "bad batch"), (dict(n=1 << 27), "bad batch"), (dict(groups=-1), "bad batch"), (dict(max_prefix=-1), "bad batch"), (dict(max_suffix=-1), "bad batch"),
     (dict(q=None), "null"), (dict(meta=None), "null"), (dict(tokens=None), "null"), (dict(off=None), "null"), (dict(lens=None), "null"),
     (dict(k=None), "null"), (dict(v=None), "null"), (dict(scratch=None), "null"), (dict(out=None), "null"),
     (dict(q=C.c_void_p(4104)), "aligned"), (dict(k=C.c_void_p(4098)), "aligned"), (dict(out=C.c_void_p(4104)), "aligned"),
