@@ -203,24 +203,35 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
 // ---------------------------------------------------------------------------------------
 
 constexpr int kSxWarps = 4;   // independent tile workers per CTA
-constexpr int kSxStages = 3;  // 16-key tiles in flight per warp
+constexpr int kSxStages = 2;  // 16-key tiles of a warp: one at work, one in flight (three CTAs to an SM)
 
 template <int D>
 constexpr size_t suffix_smem_bytes() {
   return static_cast<size_t>(kSxWarps) * kSxStages * 2 * 16 * D * sizeof(__half);
 }
 
+// The transpose of an 8x8 matrix of halves, a row's pairs in four lanes.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// The products run with the keys (then the head's dimensions) on the M axis of m16n8k16 and the query heads on
+// its N axis, 8 at a time: S^T = K Q^T and O^T += V^T P^T. With the heads on M half of each product and of O's
+// registers would be rows that no head fills.
 // CONTIG: block_size is a multiple of 16, so an aligned 16-key tile is one contiguous run of a page.
-// WIDE: more than 8 query heads per KV head (rows 8..15 of the M tile are real heads).
-// gridDim.z CTAs share the token's own keys.
-template <int D, bool CONTIG, bool WIDE>
-__global__ void __launch_bounds__(kSxWarps * 32, 2)
+// NT: groups of 8 query heads to a KV head (1 or 2). gridDim.z CTAs share the token's own keys.
+template <int D, bool CONTIG, int NT>
+__global__ void __launch_bounds__(kSxWarps * 32, NT == 1 ? 3 : 2)
 suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half* __restrict__ kc, const __half* __restrict__ vc,
               Partials part, int heads, int kv_heads, int bs, int bs_shift, int q_stride, float scale_log2e, int first) {
   constexpr int CH = D / 8;
   constexpr int TILE_HALVES = 16 * D;
+  constexpr int OS = D + 4;  // floats between heads in the exchange: they start on different banks
+  static_assert(8 * NT * OS * 4 <= kSxStages * 2 * TILE_HALVES * 2, "a warp's ring holds its output");
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  __shared__ float s_m[kSxWarps][16], s_l[kSxWarps][16];
+  __shared__ float s_m[kSxWarps][8 * NT], s_l[kSxWarps][8 * NT];
 
   // Behind a prefix kernel, all of whose CTAs have waited for what came before them, the metadata, q and the
   // pages are complete (and read from L2): nothing is waited for. Only the grid's last CTA waits, at its
@@ -248,29 +259,6 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   const int G = heads / kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, t4 = lane & 3;
-
-  // The heads' queries as A fragments: rows 0..7 hi of heads 0..7; rows 8..15 hi of heads 8..15 (then the lo
-  // halves need fragments of their own) or, with up to 8 heads, their lo, so that one product makes both.
-  uint32_t qf[D / 16][4], ql[WIDE ? D / 16 : 1][4];
-  {
-    const float* q0 = q + static_cast<long long>(tok) * q_stride + (kvh * G) * D;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d0 = kk * 16 + 2 * t4 + 8 * e;
-        float2 a = make_float2(0.f, 0.f), b = a;
-        if (gid < G) a = __ldcg(reinterpret_cast<const float2*>(q0 + gid * D + d0));
-        if constexpr (WIDE) {
-          if (gid + 8 < G) b = __ldcg(reinterpret_cast<const float2*>(q0 + (gid + 8) * D + d0));
-          split_half2(a.x, a.y, qf[kk][2 * e], ql[kk][2 * e]);
-          split_half2(b.x, b.y, qf[kk][2 * e + 1], ql[kk][2 * e + 1]);
-        } else {
-          split_half2(a.x, a.y, qf[kk][2 * e], qf[kk][2 * e + 1]);
-        }
-      }
-    }
-  }
 
   __half* ring = reinterpret_cast<__half*>(smem_raw) + static_cast<size_t>(warp) * kSxStages * 2 * TILE_HALVES;
   const uint32_t ring_u32 = smem_u32(ring);
@@ -323,10 +311,29 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
     cp_async_commit();
   }
 
-  float o[D / 8][4];
+  // The heads' queries as B fragments, hi and lo halves: head n * 8 + gid, dimensions 2 t4 and 2 t4 + 8 of each 16.
+  uint32_t qh[NT][D / 16][2], ql[NT][D / 16][2];
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float mr[2] = {-INFINITY, -INFINITY}, lr[2] = {0.f, 0.f};  // rows gid and gid + 8, log2 domain
+  for (int n = 0; n < NT; ++n) {
+    const int h = n * 8 + gid;
+    const float* q0 = q + static_cast<long long>(tok) * q_stride + (kvh * G + min(h, G - 1)) * D + 2 * t4;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(q0 + kk * 16 + 8 * e));
+        split_half2(h < G ? x.x : 0.f, h < G ? x.y : 0.f, qh[n][kk][e], ql[n][kk][e]);
+      }
+  }
+
+  float o[NT][D / 16][4];  // O^T: dimensions 16 j + gid (then + 8), heads n * 8 + 2 t4 and + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+  float mr[NT][2], lr[NT][2];  // heads n * 8 + 2 t4 and + 1, log2 domain; the sum is this lane's keys' own
+#pragma unroll
+  for (int n = 0; n < NT; ++n) mr[n][0] = mr[n][1] = -INFINITY, lr[n][0] = lr[n][1] = 0.f;
 
   for (int j = 0; j < my_tiles; ++j) {
     cp_async_wait<kSxStages - 2>();
@@ -336,72 +343,86 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
 
     const uint32_t ktile = ring_u32 + static_cast<uint32_t>(j % kSxStages) * 2 * TILE_HALVES * 2;
     const uint32_t vtile = ktile + TILE_HALVES * 2;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    qk_16x16<D>(s, qf, ktile, lane);
-    if constexpr (WIDE) {
-      qk_16x16<D>(s, ql, ktile, lane);
-    } else {
+    float s[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        s[nt][0] += s[nt][2];
-        s[nt][1] += s[nt][3];
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t ka[4];
+      ldmatrix_x4(ka, ktile + swz<CH>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4)) * 16);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_f16(s[n], ka, qh[n][kk][0], qh[n][kk][1]);
+        mma_f16(s[n], ka, ql[n][kk][0], ql[n][kk][1]);
       }
     }
 
-    const int key0 = k0 + (warp + j * kSxWarps) * 16 + 2 * t4;
-    float corr[2];
-    uint32_t pa[4] = {0u, 0u, 0u, 0u};
+    const int key = k0 + (warp + j * kSxWarps) * 16 + gid;  // of s[.][0], s[.][1]; 8 further on for the other two
+    const bool see0 = key >= start && key < k1, see1 = key + 8 >= start && key + 8 < k1;
+    uint32_t pb[NT][2];
 #pragma unroll
-    for (int r = 0; r < (WIDE ? 2 : 1); ++r) {
-      float mx = -INFINITY;
+    for (int n = 0; n < NT; ++n) {
+      float corr[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = key0 + (e >> 1) * 8 + (e & 1);
-        float& x = s[e >> 1][2 * r + (e & 1)];
-        x = key >= start && key < k1 ? x * scale_log2e : -INFINITY;
-        mx = fmaxf(mx, x);
+      for (int e = 0; e < 2; ++e) {
+        float& x0 = s[n][e];
+        float& x1 = s[n][e + 2];
+        x0 = see0 ? x0 * scale_log2e : -INFINITY;
+        x1 = see1 ? x1 * scale_log2e : -INFINITY;
+        float mx = fmaxf(x0, x1);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(mr[n][e], mx);
+        const float ref = mn == -INFINITY ? 0.f : mn;  // only masked keys so far
+        corr[e] = fast_exp2(mr[n][e] - ref);
+        mr[n][e] = mn;
+        x0 = fast_exp2(x0 - ref);
+        x1 = fast_exp2(x1 - ref);
+        lr[n][e] = lr[n][e] * corr[e] + (x0 + x1);
       }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(mr[r], mx);
-      const float ref = mn == -INFINITY ? 0.f : mn;  // only masked keys so far
-      corr[r] = fast_exp2(mr[r] - ref);
-      mr[r] = mn;
-      const float p0 = fast_exp2(s[0][2 * r] - ref), p1 = fast_exp2(s[0][2 * r + 1] - ref);
-      const float p2 = fast_exp2(s[1][2 * r] - ref), p3 = fast_exp2(s[1][2 * r + 1] - ref);
-      lr[r] = lr[r] * corr[r] + ((p0 + p1) + (p2 + p3));
-      pa[r] = pack_half2(p0, p1);
-      pa[r + 2] = pack_half2(p2, p3);
+      // weights of key gid (then gid + 8) -> weights of keys 2 t4, 2 t4 + 1 of head gid: the second product's B operand
+      pb[n][0] = transpose_8x8(pack_half2(s[n][0], s[n][1]));
+      pb[n][1] = transpose_8x8(pack_half2(s[n][2], s[n][3]));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        o[n][i][0] *= corr[0];
+        o[n][i][1] *= corr[1];
+        o[n][i][2] *= corr[0];
+        o[n][i][3] *= corr[1];
+      }
     }
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      o[i][0] *= corr[0];
-      o[i][1] *= corr[0];
-      if constexpr (WIDE) {
-        o[i][2] *= corr[1];
-        o[i][3] *= corr[1];
-      }
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t va[4];
+      ldmatrix_x4_trans(va, vtile + swz<CH>((lane & 7) + (lane >> 4) * 8, 2 * i + ((lane >> 3) & 1)) * 16);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_f16(o[n][i], va, pb[n][0], pb[n][1]);
     }
-    pv_16x16<D>(o, pa, vtile, lane);
   }
   cp_async_wait<0>();
   __syncwarp();
 
   // The warps' (m, l, o) meet in shared memory (each warp reuses its own ring).
+  float* os = reinterpret_cast<float*>(ring);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    lr[r] += __shfl_xor_sync(0xffffffffu, lr[r], 1);
-    lr[r] += __shfl_xor_sync(0xffffffffu, lr[r], 2);
-    if (t4 == 0) {
-      s_m[warp][gid + 8 * r] = mr[r];
-      s_l[warp][gid + 8 * r] = lr[r];
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      lr[n][e] += __shfl_xor_sync(0xffffffffu, lr[n][e], 4);
+      lr[n][e] += __shfl_xor_sync(0xffffffffu, lr[n][e], 8);
+      lr[n][e] += __shfl_xor_sync(0xffffffffu, lr[n][e], 16);
+      const int h = n * 8 + 2 * t4 + e;
+      if (gid == 0) {
+        s_m[warp][h] = mr[n][e];
+        s_l[warp][h] = lr[n][e];
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        os[h * OS + i * 16 + gid] = o[n][i][e];
+        os[h * OS + i * 16 + 8 + gid] = o[n][i][e + 2];
+      }
     }
-  }
-  float* os = reinterpret_cast<float*>(ring);  // [16][D] floats = 64 D bytes <= the ring's 192 D
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    *reinterpret_cast<float2*>(os + gid * D + i * 8 + 2 * t4) = make_float2(o[i][0], o[i][1]);
-    if constexpr (WIDE) *reinterpret_cast<float2*>(os + (gid + 8) * D + i * 8 + 2 * t4) = make_float2(o[i][2], o[i][3]);
   }
   __syncthreads();
 
@@ -418,7 +439,7 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
 #pragma unroll
     for (int w = 0; w < kSxWarps; ++w) {
       const float e = fast_exp2(s_m[w][r] - ref);
-      const float4 x = *reinterpret_cast<const float4*>(os_all + w * WARP_FLOATS + r * D + d);
+      const float4 x = *reinterpret_cast<const float4*>(os_all + w * WARP_FLOATS + r * OS + d);
       acc.x += e * x.x, acc.y += e * x.y, acc.z += e * x.z, acc.w += e * x.w;
       L += e * s_l[w][r];
     }
@@ -559,11 +580,11 @@ Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int
   return p;
 }
 
-template <int D, bool CONTIG, bool WIDE>
+template <int D, bool CONTIG, int NT>
 void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const __half* kc, const __half* vc,
                    const Partials& part, int slices, int first, cudaStream_t st) {
   static PerDeviceOnce once;
-  auto kernel = suffix_kernel<D, CONTIG, WIDE>;
+  auto kernel = suffix_kernel<D, CONTIG, NT>;
   if (once.first())
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(suffix_smem_bytes<D>())));
   count_launch();
@@ -589,10 +610,10 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
   }
   const bool contig = s.block_size % 16 == 0, wide = s.heads / s.kv_heads > 8;
   const int first = plan.parts == 0;
-  if (contig && !wide) launch_suffix<D, true, false>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
-  else if (contig) launch_suffix<D, true, true>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
-  else if (!wide) launch_suffix<D, false, false>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
-  else launch_suffix<D, false, true>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  if (contig && !wide) launch_suffix<D, true, 1>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  else if (contig) launch_suffix<D, true, 2>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  else if (!wide) launch_suffix<D, false, 1>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  else launch_suffix<D, false, 2>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
   count_launch();
   launch_pdl(join_kernel<D>, dim3(div_up(static_cast<long long>(gr.n_decode) * s.heads, kJoinWarps)), dim3(kJoinWarps * 32), 0, st, m, gr,
              part, out, s.heads, s.o_stride);
