@@ -125,8 +125,9 @@ adjust_logits_kernel(const LogitArgs a) {
       if (i0 == tid) __syncthreads();  // the counters are zero
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = place(id[u]);
-        if (at < 0) continue;
+        // one comparison: an id below 0 is out of reach, or a place ahead of the row, whose count nobody reads
+        const uint32_t at = static_cast<uint32_t>(id[u]) - static_cast<uint32_t>(v0);
+        if (at >= static_cast<uint32_t>(room)) continue;
         if (i0 + u * kLgThreads < prompt) atomicOr(&count[at], kSeen);
         else atomicAdd(&count[at], 1u);
       }
@@ -203,7 +204,9 @@ void launch_adjust_logits(const float* logits, int ld_logits, float* out, int ld
   if (R == 0) return;
   const LogitArgs a{logits, out, penalties, history, history_len, prompt_len, bias_ids, bias_values, bias_len, mask,
                     ld_logits, ld_out, V, ld_history, ld_bias, ld_mask};
-  // Every segment reads its row's whole history, so segments are as long as leaves two CTAs for every SM.
+  // Every segment reads its row's whole history, so segments are as long as leaves two CTAs for every SM: 256 rows of
+  // 128256 logits with 4116 tokens each take 63 us in segments of 16384, 68, 112 and 179 in 8192, 4096 and 2048.
+  // (Clusters that read a history once and count in the owner's shared memory: 119 us.)
   const long long places = V + 3LL, want = 2LL * sm_count();
   if (R * (places / (kLgThreads * 32)) >= want) launch_segments<8>(a, R, st);
   else if (R * (places / (kLgThreads * 16)) >= want) launch_segments<4>(a, R, st);

@@ -471,6 +471,11 @@ LOGIT_CASES = [
     (3, 5000, 0, 0, True),
     (3, 5000, 12, 0, False),
     (2, 300000, 50000, 1000, True),
+    # batches whose segments are long: 4 of 8192 tokens; clusters of 8, 2 x 5 and 2 segments of 16384
+    (100, 33000, 700, 3, True),
+    (48, 128256, 3000, 16, True),
+    (40, 151937, 5000, 0, False),
+    (300, 20000, 60, 2, True),
 ]
 
 
