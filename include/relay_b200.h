@@ -510,7 +510,7 @@ int rb200_argmax_rows(const float* logits, int R, int V, int32_t* token_out, flo
  * Ids outside [0, V) (padding) are passed over, as are bits behind V; a length above its leading
  * dimension counts as that, one below 0 as 0. logits and out rows are ld_logits and ld_out
  * floats apart; out may be logits itself with the same stride, any other overlap is not allowed.
- * Columns from V on are left as they were. R is at most 65535. */
+ * Columns from V on are left as they were. R is at most 65535, V at most 2^30. */
 typedef struct rb200_penalties {
   float repetition; /* > 0; 1: none */
   float presence;   /* 0: none */

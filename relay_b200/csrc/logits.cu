@@ -7,6 +7,8 @@
 // and stored. The few biases follow as a correction of what was stored, with the counters' memory
 // now holding the last entry of each biased token. At most 8 bytes per logit move, plus one bit of mask:
 // the kernel is bound by memory, and by latency for a few rows.
+#include <climits>
+
 #include "kernels.h"
 
 namespace rb200 {
@@ -121,7 +123,7 @@ adjust_logits_kernel(const LogitArgs a) {
     for (int i0 = tid; i0 - tid < len; i0 += U * kLgThreads) {
       int id[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) id[u] = i0 + u * kLgThreads < len ? h[i0 + u * kLgThreads] : -1;
+      for (int u = 0; u < U; ++u) id[u] = i0 + u * kLgThreads < len ? h[i0 + u * kLgThreads] : INT_MIN;
       if (i0 == tid) __syncthreads();  // the counters are zero
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -223,7 +225,7 @@ extern "C" int rb200_adjust_logits(const float* logits, int ld_logits, float* ou
                                    const float* bias_values, int ld_bias, const int32_t* bias_len, const uint32_t* mask, int ld_mask,
                                    void* stream) {
   return guarded([&] {
-    RB_REQUIRE(R >= 0 && R <= 65535 && V > 0, "adjust_logits: bad shape (1 to 65535 rows)");
+    RB_REQUIRE(R >= 0 && R <= 65535 && V > 0 && V <= (1 << 30), "adjust_logits: bad shape (at most 65535 rows of 2^30)");
     RB_REQUIRE(ld_logits >= V && ld_out >= V, "adjust_logits: rows shorter than the vocabulary");
     if (R == 0) return 0;
     RB_REQUIRE(logits && out, "adjust_logits: null argument");

@@ -94,7 +94,7 @@ def logits(**kw):
 
 
 @pytest.mark.parametrize("kw,text", [
-    (dict(R=-1), "bad shape"), (dict(R=65536), "bad shape"), (dict(V=0), "bad shape"), (dict(ld=99), "shorter"), (dict(ld_out=99), "shorter"),
+    (dict(R=-1), "bad shape"), (dict(R=65536), "bad shape"), (dict(V=0), "bad shape"), (dict(V=(1 << 30) + 1, ld=2 ** 31 - 1, ld_out=2 ** 31 - 1), "bad shape"), (dict(ld=99), "shorter"), (dict(ld_out=99), "shorter"),
     (dict(logits=None), "null"), (dict(out=None), "null"), (dict(out=PTR, ld_out=104), "same stride"),
     (dict(history=None), "history"), (dict(history_len=None), "history"), (dict(ld_history=-1), "negative"), (dict(ld_bias=-1), "negative"),
     (dict(values=None), "bias"), (dict(bias_len=None), "bias"), (dict(ld_mask=3), "mask"),
