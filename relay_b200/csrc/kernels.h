@@ -97,7 +97,8 @@ void launch_qkv_norm_post(const float* qkv, int qkv_stride, const float* bias, c
 size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix);
 void launch_shared_prefix_attention(const AttnShape& s, const float* q, const TokenMeta& m, const int* decode_tokens, int n_decode,
                                     const int* group_off, const int* prefix_len, int n_groups, int max_prefix, int max_suffix,
-                                    const __half* kc, const __half* vc, float* scratch, __half* out, cudaStream_t st);
+                                    const __half* kc, const __half* vc, float* scratch, size_t scratch_bytes, __half* out,
+                                    cudaStream_t st);
 
 // ---- logits.cu ----
 void launch_adjust_logits(const float* logits, int ld_logits, float* out, int ld_out, int R, int V, const rb200_penalties* penalties,

@@ -18,6 +18,12 @@
 // K and V tiles pass through one ring of slots in the order K0 V0 K1 V1 ..., each slot with its own
 // pair of barriers: a K slot is free again once its scores are made, long before V of the same tile.
 // Every wait is bounded; one that gives up records a code in the device's status word.
+//
+// Measured at head_dim 128: with 128 rows a tile takes 2300 - 2700 cycles (64 CTAs of 64 tiles: 96 us, tensor
+// pipe 64 % active), a stream's chain of Q K^T (1330, half of it for lo), softmax (2200) and P V (790) against
+// the other's. With 40 rows and 144 CTAs it reads 268 MB of keys in 53 us = 5.1 TB/s. Tried
+// and left out: one stream with the halves of a tile as separate softmax states (20 % slower), P kept in
+// registers for one pass over S (spills), sixteen softmax warps (no faster).
 #include <cuda.h>
 
 #include "attn_tiles.cuh"

@@ -131,7 +131,8 @@ def _check_meta(op: str, here: int, meta: TokenMeta, tokens: int) -> None:
 def _check_pools(op: str, here: int, page, k_pool, v_pool) -> None:
     if not _plain(here, torch.float16, k_pool, v_pool):
         _complain(op, here, ("k_pool", k_pool, torch.float16, True), ("v_pool", v_pool, torch.float16, True))
-    if k_pool.shape[1:] != page or v_pool.shape[1:] != page:
+    dims = k_pool.shape
+    if dims[1:] != page or v_pool.shape != dims:
         raise ValueError(f"{op}: the pools must be [blocks, kv_heads, block_size, head_dim] tensors")
 
 
@@ -168,9 +169,11 @@ def shared_prefix_attention(shape: CAttnShape, q: torch.Tensor, meta: TokenMeta,
     if group_off.numel() != n_groups + 1:
         raise ValueError(f"{op}: group_off must have one entry more than prefix_len")
     width = shape.heads * shape.head_dim
-    if q.dim() != 2 or q.size(0) < rows or q.size(1) < width or (rows > 1 and q.stride(0) != shape.q_stride):
+    dims = q.shape
+    if len(dims) != 2 or dims[0] < rows or dims[1] < width or (rows > 1 and q.stride(0) != shape.q_stride):
         raise ValueError(f"{op}: q must have the batch's rows, {shape.q_stride} values apart")
-    if out.dim() != 2 or out.size(0) < rows or out.size(1) < width or (rows > 1 and out.stride(0) != shape.o_stride):
+    dims = out.shape
+    if len(dims) != 2 or dims[0] < rows or dims[1] < width or (rows > 1 and out.stride(0) != shape.o_stride):
         raise ValueError(f"{op}: out must have the batch's rows, {shape.o_stride} values apart")
     L, sh, m = _lib.lib(), C.byref(shape), meta.c()
     if scratch is None:
@@ -261,10 +264,11 @@ def qkv_norm_post(qkv, bias, q_norm, k_norm, eps, inv_freq, meta: TokenMeta, q_o
         _complain(op, here, ("qkv", qkv, f32, False), ("bias", bias, f32, True), ("q_norm", q_norm, f32, True),
                   ("k_norm", k_norm, f32, True), ("inv_freq", inv_freq, f32, True), ("q_out", q_out, f32, False))
     width = (heads + 2 * kv_heads) * head_dim
-    if qkv.dim() != 2 or qkv.size(1) < width:
+    dims, q_dims = qkv.shape, q_out.shape
+    if len(dims) != 2 or dims[1] < width:
         raise ValueError(f"{op}: qkv must be [tokens, (heads + 2 kv_heads) head_dim]")
-    T = qkv.size(0)
-    if q_out.dim() != 2 or q_out.size(0) < T or q_out.size(1) < heads * head_dim:
+    T = dims[0]
+    if len(q_dims) != 2 or q_dims[0] < T or q_dims[1] < heads * head_dim:
         raise ValueError(f"{op}: q_out must be [tokens, heads head_dim]")
     _check_meta(op, here, meta, T)
     _check_pools(op, here, (kv_heads, block_size, head_dim), k_pool, v_pool)
