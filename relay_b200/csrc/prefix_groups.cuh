@@ -33,6 +33,13 @@ struct Partials {
 
 __device__ __forceinline__ int slice_of(int P, int parts) { return (((P + parts - 1) / parts) + kPrefixSlice - 1) / kPrefixSlice * kPrefixSlice; }
 
+// How many of them a prefix of P keys fills.
+__device__ __forceinline__ int slices_used(int P, int parts) {
+  if (P <= 0) return 0;
+  const int slice = slice_of(P, parts);
+  return (P + slice - 1) / slice;
+}
+
 // How many keys the entries [lo, hi) of group g share, and (`with_table`) the block table that names them.
 struct Prefix {
   int keys;

@@ -14,8 +14,9 @@
 //    tensor cores where many tokens share, by memory where few do;
 //  * suffix_kernel: a CTA takes one token and KV head and a slice of the token's own keys, and leaves a
 //    partial per head. Bound by memory (alone, 256 tokens with 128 - 640 keys of 8 x 128: 407 MB in 70 us =
-//    5.8 TB/s). It needs nothing of the first kernel and runs beside it, on the SMs that one leaves free;
-//  * join_kernel: a warp takes one token and head and adds its partials. Bound by latency.
+//    5.8 TB/s). Its keys need nothing of the first kernel: it runs beside it, on the SMs that one leaves free,
+//    and in a small batch (`finish`) then waits for it and adds its partials;
+//  * join_kernel, in larger batches: a warp takes one token and head and adds its partials. Bound by latency.
 //
 // Scores take q in full (two fp16 halves, split_half2); the weights round to fp16 for the second product.
 #include "attn_tiles.cuh"
@@ -225,7 +226,8 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 template <int D, bool CONTIG, int NT>
 __global__ void __launch_bounds__(kSxWarps * 32, NT == 1 ? 3 : 2)
 suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half* __restrict__ kc, const __half* __restrict__ vc,
-              Partials part, int heads, int kv_heads, int bs, int bs_shift, int q_stride, float scale_log2e, int first) {
+              Partials part, __half* __restrict__ out, int heads, int kv_heads, int bs, int bs_shift, int q_stride, int o_stride,
+              float scale_log2e, int first, int finish) {
   constexpr int CH = D / 8;
   constexpr int TILE_HALVES = 16 * D;
   constexpr int OS = D + 4;  // floats between heads in the exchange: they start on different banks
@@ -234,8 +236,9 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   __shared__ float s_m[kSxWarps][8 * NT], s_l[kSxWarps][8 * NT];
 
   // Behind a prefix kernel, all of whose CTAs have waited for what came before them, the metadata, q and the
-  // pages are complete (and read from L2): nothing is waited for. Only the grid's last CTA waits, at its
-  // end, so that this kernel is not complete before the one ahead of it is. `first`: there is none.
+  // pages are complete (and read from L2): nothing is waited for until the keys are done. Then every CTA waits
+  // for the shared part (`finish`) or only the grid's last one, so that this kernel is not complete before the one
+  // ahead of it is. `first`: there is none.
   if (first) pdl_wait();
   pdl_trigger();
   const bool last = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
@@ -424,10 +427,12 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
       }
     }
   }
+  if (finish) pdl_wait();
   __syncthreads();
 
   const float* os_all = reinterpret_cast<const float*>(smem_raw);
   constexpr int WARP_FLOATS = kSxStages * TILE_HALVES;  // ring size of one warp in floats
+  const int used = slices_used(P, part.parts);
   for (int idx = threadIdx.x; idx < G * D / 4; idx += blockDim.x) {
     const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
     float M = s_m[0][r];
@@ -443,11 +448,42 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
       acc.x += e * x.x, acc.y += e * x.y, acc.z += e * x.z, acc.w += e * x.w;
       L += e * s_l[w][r];
     }
-    const long long at = (static_cast<long long>(di) * heads + kvh * G + r) * part.total + part.parts + rank;
-    *reinterpret_cast<float4*>(part.o + at * D + d) = acc;
-    if (d == 0) *reinterpret_cast<float2*>(part.ml + at * 2) = make_float2(M, L);
+    const long long at = (static_cast<long long>(di) * heads + kvh * G + r) * part.total;
+    if (!finish) {
+      *reinterpret_cast<float4*>(part.o + (at + part.parts + rank) * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(part.ml + (at + part.parts + rank) * 2) = make_float2(M, L);
+      continue;
+    }
+    // the shared part's partials of this head, U at a time, in the order of the slices
+    constexpr int U = 8;
+    for (int p0 = 0; p0 < used; p0 += U) {
+      float2 ml[U];
+      float4 x[U];
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool there = p0 + u < used;
+        ml[u] = there ? *reinterpret_cast<const float2*>(part.ml + (at + p0 + u) * 2) : make_float2(-INFINITY, 0.f);
+        x[u] = there ? *reinterpret_cast<const float4*>(part.o + (at + p0 + u) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u].x);
+      const float to = top == -INFINITY ? 0.f : top, e = fast_exp2(M - to);
+      acc.x *= e, acc.y *= e, acc.z *= e, acc.w *= e;
+      L *= e;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = fast_exp2(ml[u].x - to);
+        acc.x += w * x[u].x, acc.y += w * x[u].y, acc.z += w * x[u].z, acc.w += w * x[u].w;
+        L += w * ml[u].y;
+      }
+      M = top;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;  // no key at all: zeros
+    *reinterpret_cast<uint2*>(out + static_cast<long long>(tok) * o_stride + (kvh * G + r) * D + d) =
+        make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
   }
-  if (last) pdl_wait();
+  if (last && !finish) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------
@@ -472,7 +508,7 @@ join_kernel(TokenMeta m, Groups gr, Partials part, __half* __restrict__ out, int
   const RowTile rt = group_of(gr, di);
   const bool live = tok >= 0 && rt.g >= 0 && pair == blockIdx.x * kJoinWarps + warp;
   const int P = live ? prefix_of(gr, m, rt.g, rt.lo, rt.hi, false).keys : 0;
-  const int used = P > 0 ? (P + slice_of(P, part.parts) - 1) / slice_of(P, part.parts) : 0;  // slices of the shared keys
+  const int used = slices_used(P, part.parts);
   pdl_wait();
   if (!live) return;
   const long long base = static_cast<long long>(pair) * part.total;
@@ -539,8 +575,14 @@ long long row_tiles(const AttnShape& s, int n_decode, int n_groups, int rows) {
 }
 
 // How a call is split: row tiles, slices of the longest prefix and of a token's own keys.
+// `finish`: the suffix kernel joins the shared part itself, without a third kernel, where each (token, KV head) is one
+// CTA and all of them have a place beside the prefix kernel (two on an SM, where its CTAs of tcgen05 take both and the
+// others one): none that waits for the shared part keeps another from its keys. Measured: 4 tokens behind 500 keys, 10.7 us
+// against 11.5 with the third kernel, and 2.5 us less of the caller's time; 32 tokens behind 4096 keys, whose 256 CTAs do
+// not fit beside it, 24.0 against 20.6.
 struct Plan {
   int rows, tiles, parts, slices;
+  bool finish;
 };
 
 // The number of slices of the shared keys follows from an estimate of the call's time for each, in us: a CTA of
@@ -552,7 +594,8 @@ struct Plan {
 constexpr double kTileUs = 1.3, kStartUs = 6.0, kBytesPerUs = 5.5e6, kBytesPerSmUs = 4.2e4;
 
 Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
-  Plan p{0, 0, 0, 1};
+  Plan p{0, 0, 0, 1, false};
+  long long places = 2LL * sm_count();
   const double own_us = 0.6 * 4.0 * max_suffix * s.D * s.kv_heads * n_decode / kBytesPerUs;
   if (max_prefix > 0) {
     // 64 rows where the average group has no more
@@ -572,24 +615,28 @@ Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int
         p.parts = n;
       }
     }
+    places -= (umma_prefix_usable(s) ? 2 : 1) * ctas * p.parts;
   }
   // A few tokens with many keys of their own: slices of at least 128 keys, two CTAs for every SM.
   const long long pairs = static_cast<long long>(n_decode) * s.kv_heads;
   const long long slices = std::min<long long>(2LL * sm_count() / pairs, max_suffix / 128);
   p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(slices, kMostParts)));
+  p.finish = p.slices == 1 && pairs <= places;
   return p;
 }
 
 template <int D, bool CONTIG, int NT>
 void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const __half* kc, const __half* vc,
-                   const Partials& part, int slices, int first, cudaStream_t st) {
+                   const Partials& part, __half* out, const Plan& plan, cudaStream_t st) {
   static PerDeviceOnce once;
   auto kernel = suffix_kernel<D, CONTIG, NT>;
   if (once.first())
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(suffix_smem_bytes<D>())));
   count_launch();
-  launch_pdl(kernel, dim3(gr.n_decode, s.kv_heads, slices), dim3(kSxWarps * 32), suffix_smem_bytes<D>(), st, q, m, gr, kc, vc, part,
-             s.heads, s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, kLog2e / sqrtf(static_cast<float>(D)), first);
+  const int first = plan.parts == 0, finish = plan.finish;
+  launch_pdl(kernel, dim3(gr.n_decode, s.kv_heads, plan.slices), dim3(kSxWarps * 32), suffix_smem_bytes<D>(), st, q, m, gr, kc, vc, part,
+             out, s.heads, s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, s.o_stride, kLog2e / sqrtf(static_cast<float>(D)),
+             first, finish);
 }
 
 template <int D>
@@ -609,11 +656,11 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
     }
   }
   const bool contig = s.block_size % 16 == 0, wide = s.heads / s.kv_heads > 8;
-  const int first = plan.parts == 0;
-  if (contig && !wide) launch_suffix<D, true, 1>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
-  else if (contig) launch_suffix<D, true, 2>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
-  else if (!wide) launch_suffix<D, false, 1>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
-  else launch_suffix<D, false, 2>(s, q, m, gr, kc, vc, part, plan.slices, first, st);
+  if (contig && !wide) launch_suffix<D, true, 1>(s, q, m, gr, kc, vc, part, out, plan, st);
+  else if (contig) launch_suffix<D, true, 2>(s, q, m, gr, kc, vc, part, out, plan, st);
+  else if (!wide) launch_suffix<D, false, 1>(s, q, m, gr, kc, vc, part, out, plan, st);
+  else launch_suffix<D, false, 2>(s, q, m, gr, kc, vc, part, out, plan, st);
+  if (plan.finish) return;
   count_launch();
   launch_pdl(join_kernel<D>, dim3(div_up(static_cast<long long>(gr.n_decode) * s.heads, kJoinWarps)), dim3(kJoinWarps * 32), 0, st, m, gr,
              part, out, s.heads, s.o_stride);

@@ -324,6 +324,11 @@ PREFIX_CASES = [
     (128, 8, 2, 16, [(0, [1, 5000])]),                         # nothing shared, long own contexts
     (64, 4, 4, 16, [(0, [1])]),
     (128, 4, 1, 16, [(40000, [2500])]),
+    # few tokens behind a prefix of many slices, no long own part
+    (128, 4, 1, 16, [(40000, [100, 7])]),
+    (64, 16, 1, 16, [(9000, [3, None, -8990, 60, -8001]), (2, [1])]),
+    (32, 8, 1, 8, [(20000, [90, 1]), (5, [5])]),
+    (16, 4, 1, 16, [(8200, [1, 120, -8200])]),
 ]
 
 
