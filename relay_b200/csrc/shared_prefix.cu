@@ -203,12 +203,11 @@ prefix_mma_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __h
 // Each sequence's own keys
 // ---------------------------------------------------------------------------------------
 
-constexpr int kSxWarps = 4;   // independent tile workers per CTA
-constexpr int kSxStages = 2;  // 16-key tiles of a warp: one at work, one in flight (three CTAs to an SM)
-
-template <int D>
+// W warps to a CTA, each with a ring of S 16-key tiles: one at work, the others in flight. 4 and 2 (three CTAs to an SM)
+// where there are CTAs enough to fill the GPU, 8 and 3 where each has an SM to itself.
+template <int D, int W, int S>
 constexpr size_t suffix_smem_bytes() {
-  return static_cast<size_t>(kSxWarps) * kSxStages * 2 * 16 * D * sizeof(__half);
+  return static_cast<size_t>(W) * S * 2 * 16 * D * sizeof(__half);
 }
 
 // The transpose of an 8x8 matrix of halves, a row's pairs in four lanes.
@@ -223,17 +222,17 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 // registers would be rows that no head fills.
 // CONTIG: block_size is a multiple of 16, so an aligned 16-key tile is one contiguous run of a page.
 // NT: groups of 8 query heads to a KV head (1 or 2). gridDim.z CTAs share the token's own keys.
-template <int D, bool CONTIG, int NT>
-__global__ void __launch_bounds__(kSxWarps * 32, NT == 1 ? 3 : 2)
+template <int D, bool CONTIG, int NT, int W, int S>
+__global__ void __launch_bounds__(W * 32, W == 8 ? 1 : NT == 1 ? 3 : 2)
 suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half* __restrict__ kc, const __half* __restrict__ vc,
               Partials part, __half* __restrict__ out, int heads, int kv_heads, int bs, int bs_shift, int q_stride, int o_stride,
               float scale_log2e, int first, int finish) {
   constexpr int CH = D / 8;
   constexpr int TILE_HALVES = 16 * D;
   constexpr int OS = D + 4;  // floats between heads in the exchange: they start on different banks
-  static_assert(8 * NT * OS * 4 <= kSxStages * 2 * TILE_HALVES * 2, "a warp's ring holds its output");
+  static_assert(8 * NT * OS * 4 <= S * 2 * TILE_HALVES * 2, "a warp's ring holds its output");
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  __shared__ float s_m[kSxWarps][8 * NT], s_l[kSxWarps][8 * NT];
+  __shared__ float s_m[W][8 * NT], s_l[W][8 * NT];
 
   // Behind a prefix kernel, all of whose CTAs have waited for what came before them, the metadata, q and the
   // pages are complete (and read from L2): nothing is waited for until the keys are done. Then every CTA waits
@@ -263,20 +262,20 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, t4 = lane & 3;
 
-  __half* ring = reinterpret_cast<__half*>(smem_raw) + static_cast<size_t>(warp) * kSxStages * 2 * TILE_HALVES;
+  __half* ring = reinterpret_cast<__half*>(smem_raw) + static_cast<size_t>(warp) * S * 2 * TILE_HALVES;
   const uint32_t ring_u32 = smem_u32(ring);
-  // Tiles warp, warp + 4, ... of the slice belong to this warp. Where a tile lies in one page, its
+  // Tiles warp, warp + W, ... of the slice belong to this warp. Where a tile lies in one page, its
   // block id waits in a register: 32 tiles' ids at a time, one per lane, the next 32 on their way.
-  const int my_tiles = ntiles > warp ? (ntiles - warp + kSxWarps - 1) / kSxWarps : 0;
+  const int my_tiles = ntiles > warp ? (ntiles - warp + W - 1) / W : 0;
   auto fetch_ids = [&](int j0) {
-    const int j = j0 + lane, key = k0 + (warp + j * kSxWarps) * 16;
+    const int j = j0 + lane, key = k0 + (warp + j * W) * 16;
     return CONTIG && j < my_tiles ? __ldcg(table + (bs_shift >= 0 ? key >> bs_shift : key / bs)) : 0;
   };
   int ids = fetch_ids(0), ids_next = fetch_ids(32);
   auto load_tile = [&](int j) {
-    const uint32_t kdst = ring_u32 + static_cast<uint32_t>(j % kSxStages) * 2 * TILE_HALVES * 2;
+    const uint32_t kdst = ring_u32 + static_cast<uint32_t>(j % S) * 2 * TILE_HALVES * 2;
     const uint32_t vdst = kdst + TILE_HALVES * 2;
-    const int key0 = k0 + (warp + j * kSxWarps) * 16;
+    const int key0 = k0 + (warp + j * W) * 16;
     const int nvalid = min(16, k1 - key0);
     if constexpr (CONTIG) {
       if (j > 0 && (j & 31) == 0) {
@@ -309,8 +308,8 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   };
 
 #pragma unroll
-  for (int s = 0; s < kSxStages - 1; ++s) {
-    if (s < my_tiles) load_tile(s);
+  for (int st = 0; st < S - 1; ++st) {
+    if (st < my_tiles) load_tile(st);
     cp_async_commit();
   }
 
@@ -339,12 +338,12 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   for (int n = 0; n < NT; ++n) mr[n][0] = mr[n][1] = -INFINITY, lr[n][0] = lr[n][1] = 0.f;
 
   for (int j = 0; j < my_tiles; ++j) {
-    cp_async_wait<kSxStages - 2>();
+    cp_async_wait<S - 2>();
     __syncwarp();
-    if (j + kSxStages - 1 < my_tiles) load_tile(j + kSxStages - 1);
+    if (j + S - 1 < my_tiles) load_tile(j + S - 1);
     cp_async_commit();
 
-    const uint32_t ktile = ring_u32 + static_cast<uint32_t>(j % kSxStages) * 2 * TILE_HALVES * 2;
+    const uint32_t ktile = ring_u32 + static_cast<uint32_t>(j % S) * 2 * TILE_HALVES * 2;
     const uint32_t vtile = ktile + TILE_HALVES * 2;
     float s[NT][4];
 #pragma unroll
@@ -360,7 +359,7 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
       }
     }
 
-    const int key = k0 + (warp + j * kSxWarps) * 16 + gid;  // of s[.][0], s[.][1]; 8 further on for the other two
+    const int key = k0 + (warp + j * W) * 16 + gid;  // of s[.][0], s[.][1]; 8 further on for the other two
     const bool see0 = key >= start && key < k1, see1 = key + 8 >= start && key + 8 < k1;
     uint32_t pb[NT][2];
 #pragma unroll
@@ -431,18 +430,18 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
   __syncthreads();
 
   const float* os_all = reinterpret_cast<const float*>(smem_raw);
-  constexpr int WARP_FLOATS = kSxStages * TILE_HALVES;  // ring size of one warp in floats
+  constexpr int WARP_FLOATS = S * TILE_HALVES;  // ring size of one warp in floats
   const int used = slices_used(P, part.parts);
   for (int idx = threadIdx.x; idx < G * D / 4; idx += blockDim.x) {
     const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
     float M = s_m[0][r];
 #pragma unroll
-    for (int w = 1; w < kSxWarps; ++w) M = fmaxf(M, s_m[w][r]);
+    for (int w = 1; w < W; ++w) M = fmaxf(M, s_m[w][r]);
     const float ref = M == -INFINITY ? 0.f : M;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSxWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float e = fast_exp2(s_m[w][r] - ref);
       const float4 x = *reinterpret_cast<const float4*>(os_all + w * WARP_FLOATS + r * OS + d);
       acc.x += e * x.x, acc.y += e * x.y, acc.z += e * x.z, acc.w += e * x.w;
@@ -575,66 +574,102 @@ long long row_tiles(const AttnShape& s, int n_decode, int n_groups, int rows) {
 }
 
 // How a call is split: row tiles, slices of the longest prefix and of a token's own keys.
-// `finish`: the suffix kernel joins the shared part itself, without a third kernel, where each (token, KV head) is one
-// CTA and all of them have a place beside the prefix kernel (two on an SM, where its CTAs of tcgen05 take both and the
-// others one): none that waits for the shared part keeps another from its keys. Measured: 4 tokens behind 500 keys, 10.7 us
-// against 11.5 with the third kernel, and 2.5 us less of the caller's time; 32 tokens behind 4096 keys, whose 256 CTAs do
-// not fit beside it, 24.0 against 20.6.
+//  * `parts` 0: nothing is read as shared. A few tokens behind a short prefix are done sooner when each reads all of its
+//    keys, from L2 but for the first.
+//  * `finish`: the suffix kernel joins the shared part itself, without a third kernel, where each (token, KV head) is one
+//    CTA and all of them have a place beside the prefix kernel (two on an SM, where its CTAs of tcgen05 take both and the
+//    others one): none that waits for the shared part keeps another from its keys. Measured: 32 tokens behind 4096 keys,
+//    whose 256 CTAs do not fit beside it, 24.0 us against 20.6 with the third kernel; 48 tokens of 4 KV heads of 32 in two
+//    groups of 777 and 300 keys 9.9 against 11.0.
+//  * `wide`: CTAs of eight warps in the suffix kernel, where each has an SM to itself.
 struct Plan {
   int rows, tiles, parts, slices;
-  bool finish;
+  bool finish, wide;
 };
 
-// The number of slices of the shared keys follows from an estimate of the call's time for each, in us: a CTA of
-// the prefix kernel takes kTileUs for every 128 keys and kStartUs besides; the own keys (six tenths of the
-// most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel leaves
-// free get kBytesPerSmUs each until it ends. Measured at 32 + 2 x 8 heads of 128: 256 tokens behind 8192 keys
-// with 128 - 640 of their own, 108 us in one slice (64 CTAs beside the own keys) and 120 in two, which fill the
-// GPU; 32 tokens behind 4096 with 64 - 512: 25, 22, 26 and 27 us in 4, 8, 11 and 16 slices.
-constexpr double kTileUs = 1.3, kStartUs = 6.0, kBytesPerUs = 5.5e6, kBytesPerSmUs = 4.2e4;
+// The plan follows from estimates in us:
+//  * a CTA of the prefix kernel takes kTileUs for every 128 keys and kStartUs besides, and the join kJoinUs; the own keys
+//    (six tenths of the most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel
+//    leaves free get kBytesPerSmUs each until it ends. Measured at 32 + 2 x 8 heads of 128: 256 tokens behind 8192 keys
+//    with 128 - 640 of their own, 108 us in one slice (64 CTAs beside the own keys) and 120 in two, which fill the
+//    GPU; 32 tokens behind 4096 with 64 - 512: 25, 22, 26 and 27 us in 4, 8, 11 and 16 slices;
+//  * the suffix kernel takes kOwnStartUs and for every key of a slice 5 ns and 35 ps a value of the head (blocks that
+//    16 keys do not divide: 2.5 ns more), 0.6 of that in CTAs of eight warps (`wide`), and where there are more CTAs than
+//    SMs eight tenths of it times the CTAs to an SM; slices take kOwnJoinUs more;
+//  * a launch behind the first counts kLaunchUs, of the 2.5 us of the caller's time for it that a graph does not spend.
+// Measured over 150 batches of 1 - 48 tokens behind 100 - 3000 keys in five head layouts: all keys as the tokens' own
+// 5.1 us against 10.3 shared at 16 tokens of 8 KV heads of 128 behind 100 keys, 7.8 against 10.8 behind 500, 21 against
+// 14 behind 3000; one token behind 500 keys 6.9 against 8.5 in CTAs of four warps.
+constexpr double kTileUs = 1.3, kStartUs = 6.0, kJoinUs = 1.5, kBytesPerUs = 5.5e6, kBytesPerSmUs = 4.2e4;
+constexpr double kOwnStartUs = 3.8, kOwnJoinUs = 2.0, kLaunchUs = 2.0;
 
-Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
-  Plan p{0, 0, 0, 1, false};
-  long long places = 2LL * sm_count();
-  const double own_us = 0.6 * 4.0 * max_suffix * s.D * s.kv_heads * n_decode / kBytesPerUs;
-  if (max_prefix > 0) {
-    // 64 rows where the average group has no more
-    p.rows = umma_prefix_usable(s) && static_cast<long long>(n_decode) * (s.heads / s.kv_heads) > 64LL * n_groups ? 128 : 64;
-    p.tiles = static_cast<int>(row_tiles(s, n_decode, n_groups, p.rows));
-    const long long ctas = static_cast<long long>(p.tiles) * s.kv_heads;
-    const long long slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();  // one CTA of the tcgen05 kernel fits an SM
-    double least = -1.0;
-    for (int n = 1; n <= kMostParts && (n == 1 || max_prefix > (n - 1) * 2 * kPrefixSlice); ++n) {
-      const double waves = static_cast<double>((ctas * n + slots - 1) / slots);
-      const double shared_us = waves * (div_up(div_up(max_prefix, n), kPrefixSlice) * kTileUs + kStartUs);
-      const double idle = std::max<double>(0.0, 1.0 - static_cast<double>(ctas * n) / slots) * sm_count();
-      const double beside = shared_us * std::min(1.0, idle * kBytesPerSmUs / kBytesPerUs);
-      const double us = shared_us + std::max(0.0, own_us - beside);
-      if (least < 0.0 || us < least) {
-        least = us;
-        p.parts = n;
-      }
-    }
-    places -= (umma_prefix_usable(s) ? 2 : 1) * ctas * p.parts;
-  }
-  // A few tokens with many keys of their own: slices of at least 128 keys, two CTAs for every SM.
-  const long long pairs = static_cast<long long>(n_decode) * s.kv_heads;
-  const long long slices = std::min<long long>(2LL * sm_count() / pairs, max_suffix / 128);
-  p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(slices, kMostParts)));
-  p.finish = p.slices == 1 && pairs <= places;
-  return p;
+double own_us(const AttnShape& s, long long pairs, double keys, int slices, bool wide) {
+  const double key_us = (0.005 + 35e-6 * s.D + (s.block_size % 16 == 0 ? 0.0 : 0.0025)) * (wide ? 0.6 : 1.0);
+  const double load = 0.8 * static_cast<double>(pairs * slices) / sm_count();
+  return kOwnStartUs + keys / slices * key_us * std::max(1.0, load) + (slices > 1 ? kOwnJoinUs + kLaunchUs : 0.0);
 }
 
-template <int D, bool CONTIG, int NT>
+Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
+  const long long pairs = static_cast<long long>(n_decode) * s.kv_heads;
+  // Slices of own keys: at least 128 keys each, two CTAs for every SM.
+  auto most_slices = [&](double keys) {
+    const double most = std::min<double>(2.0 * sm_count() / static_cast<double>(pairs), keys / 128.0);
+    return static_cast<int>(std::max(1.0, std::min<double>(most, kMostParts)));
+  };
+
+  // every key as the token's own
+  Plan alone{0, 0, 0, 1, true, false};
+  const double keys = static_cast<double>(max_prefix) + max_suffix;
+  double alone_us = -1.0;
+  for (int n = 1; n <= most_slices(keys); ++n) {
+    const bool wide = pairs * n <= sm_count();
+    const double us = own_us(s, pairs, keys, n, wide);
+    if (alone_us < 0.0 || us < alone_us) {
+      alone_us = us;
+      alone.slices = n;
+      alone.finish = n == 1;
+      alone.wide = wide;
+    }
+  }
+  if (max_prefix == 0) return alone;
+
+  Plan p{0, 0, 1, 1, false, false};
+  // 64 rows where the average group has no more
+  p.rows = umma_prefix_usable(s) && static_cast<long long>(n_decode) * (s.heads / s.kv_heads) > 64LL * n_groups ? 128 : 64;
+  p.tiles = static_cast<int>(row_tiles(s, n_decode, n_groups, p.rows));
+  const long long ctas = static_cast<long long>(p.tiles) * s.kv_heads;
+  const long long slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();  // one CTA of the tcgen05 kernel fits an SM
+  const double suffix_us = 0.6 * 4.0 * max_suffix * s.D * static_cast<double>(pairs) / kBytesPerUs;
+  double least = -1.0, prefix_us = 0.0;
+  for (int n = 1; n <= kMostParts && (n == 1 || max_prefix > (n - 1) * 2 * kPrefixSlice); ++n) {
+    const double waves = static_cast<double>((ctas * n + slots - 1) / slots);
+    const double shared_us = waves * (div_up(div_up(max_prefix, n), kPrefixSlice) * kTileUs + kStartUs);
+    const double idle = std::max<double>(0.0, 1.0 - static_cast<double>(ctas * n) / slots) * sm_count();
+    const double beside = shared_us * std::min(1.0, idle * kBytesPerSmUs / kBytesPerUs);
+    const double us = shared_us + std::max(0.0, suffix_us - beside);
+    if (least < 0.0 || us < least) {
+      least = us;
+      prefix_us = shared_us;
+      p.parts = n;
+    }
+  }
+  // own keys that one CTA of each pair reads beside the prefix kernel need no slices
+  const bool beside = pairs <= 2LL * sm_count() - (umma_prefix_usable(s) ? 2 : 1) * ctas * p.parts;
+  p.slices = beside && own_us(s, pairs, max_suffix, 1, false) <= prefix_us ? 1 : most_slices(max_suffix);
+  p.finish = beside && p.slices == 1;
+  return alone_us <= least + kJoinUs + (p.finish ? 1 : 2) * kLaunchUs ? alone : p;
+}
+
+template <int D, bool CONTIG, int NT, int W, int S>
 void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const Groups& gr, const __half* kc, const __half* vc,
                    const Partials& part, __half* out, const Plan& plan, cudaStream_t st) {
   static PerDeviceOnce once;
-  auto kernel = suffix_kernel<D, CONTIG, NT>;
+  auto kernel = suffix_kernel<D, CONTIG, NT, W, S>;
   if (once.first())
-    RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(suffix_smem_bytes<D>())));
+    RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(suffix_smem_bytes<D, W, S>())));
   count_launch();
   const int first = plan.parts == 0, finish = plan.finish;
-  launch_pdl(kernel, dim3(gr.n_decode, s.kv_heads, plan.slices), dim3(kSxWarps * 32), suffix_smem_bytes<D>(), st, q, m, gr, kc, vc, part,
+  launch_pdl(kernel, dim3(gr.n_decode, s.kv_heads, plan.slices), dim3(W * 32), suffix_smem_bytes<D, W, S>(), st, q, m, gr, kc, vc, part,
              out, s.heads, s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, s.o_stride, kLog2e / sqrtf(static_cast<float>(D)),
              first, finish);
 }
@@ -656,25 +691,34 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
     }
   }
   const bool contig = s.block_size % 16 == 0, wide = s.heads / s.kv_heads > 8;
-  if (contig && !wide) launch_suffix<D, true, 1>(s, q, m, gr, kc, vc, part, out, plan, st);
-  else if (contig) launch_suffix<D, true, 2>(s, q, m, gr, kc, vc, part, out, plan, st);
-  else if (!wide) launch_suffix<D, false, 1>(s, q, m, gr, kc, vc, part, out, plan, st);
-  else launch_suffix<D, false, 2>(s, q, m, gr, kc, vc, part, out, plan, st);
+  auto launch = [&](auto contig_, auto nt) {
+    constexpr bool CONTIG = decltype(contig_)::value;
+    constexpr int NT = decltype(nt)::value;
+    if (plan.wide) launch_suffix<D, CONTIG, NT, 8, 3>(s, q, m, gr, kc, vc, part, out, plan, st);
+    else launch_suffix<D, CONTIG, NT, 4, 2>(s, q, m, gr, kc, vc, part, out, plan, st);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (contig && !wide) launch(std::true_type{}, One{});
+  else if (contig) launch(std::true_type{}, Two{});
+  else if (!wide) launch(std::false_type{}, One{});
+  else launch(std::false_type{}, Two{});
   if (plan.finish) return;
   count_launch();
   launch_pdl(join_kernel<D>, dim3(div_up(static_cast<long long>(gr.n_decode) * s.heads, kJoinWarps)), dim3(kJoinWarps * 32), 0, st, m, gr,
              part, out, s.heads, s.o_stride);
 }
 
-size_t scratch_of(const AttnShape& s, int n_decode, const Plan& p) {
-  return static_cast<size_t>(n_decode) * s.heads * (p.parts + p.slices) * (s.D + 2) * sizeof(float);
+// Room for a partial of the shared keys where there may be some, whatever the plan.
+size_t scratch_of(const AttnShape& s, int n_decode, int max_prefix, const Plan& p) {
+  return static_cast<size_t>(n_decode) * s.heads * (std::max(p.parts, max_prefix > 0 ? 1 : 0) + p.slices) * (s.D + 2) * sizeof(float);
 }
 
 }  // namespace
 
 size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
   if (n_decode <= 0 || n_groups <= 0) return 0;
-  return scratch_of(s, n_decode, plan_of(s, n_decode, n_groups, max_prefix, max_suffix));
+  return scratch_of(s, n_decode, max_prefix, plan_of(s, n_decode, n_groups, max_prefix, max_suffix));
 }
 
 void launch_shared_prefix_attention(const AttnShape& s, const float* q, const TokenMeta& m, const int* decode_tokens, int n_decode,
@@ -683,7 +727,7 @@ void launch_shared_prefix_attention(const AttnShape& s, const float* q, const To
                                     cudaStream_t st) {
   if (n_decode == 0) return;
   const Plan plan = plan_of(s, n_decode, n_groups, max_prefix, max_suffix);
-  RB_REQUIRE(scratch_bytes >= scratch_of(s, n_decode, plan), "shared prefix attention: scratch too small");
+  RB_REQUIRE(scratch_bytes >= scratch_of(s, n_decode, max_prefix, plan), "shared prefix attention: scratch too small");
   const Groups gr{decode_tokens, group_off, plan.parts > 0 ? prefix_len : nullptr, n_decode, n_groups};
   Partials part;
   part.parts = plan.parts;

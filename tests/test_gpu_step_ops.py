@@ -298,6 +298,15 @@ def run_prefix(ops, c, hints=None, scratch=None, out=None, pools=None):
     return out.cpu().numpy()
 
 
+# Lengths for the plan behind which no prefix is short enough to be read as each token's own, and is split into slices of
+# 128 keys; and more padding than tokens, behind which its slices are few.
+SHARED = (1 << 20, 0)
+
+
+def padded(c, entries=3000):
+    return dict(c, tokens=np.concatenate([c["tokens"], np.full(entries, -1, np.int32)]))
+
+
 PREFIX_CASES = [
     # D, heads, kv_heads, bs, groups
     (128, 32, 8, 16, [(500, [1, 7, 16, 40])]),
@@ -340,11 +349,24 @@ def test_shared_prefix_attention(ops, D, heads, kv_heads, bs, groups):
     assert np.array_equal(out, run_prefix(ops, c))  # the same bits on every run
 
 
+@pytest.mark.parametrize("slices", ["many", "few"])
+@pytest.mark.parametrize("D,heads,kv_heads,bs,groups", PREFIX_CASES)
+def test_shared_prefix_attention_read_as_shared(ops, D, heads, kv_heads, bs, groups, slices):
+    c = prefix_case(D + len(groups), D, heads, kv_heads, bs, groups)
+    run = (lambda: run_prefix(ops, c, SHARED)) if slices == "many" else (lambda: run_prefix(ops, padded(c)))
+    out = run()
+    check_prefix(c, out, 7.0)
+    assert np.array_equal(out, run())
+
+
+@pytest.mark.parametrize("hints", [None, SHARED])
 @pytest.mark.parametrize("D,heads,kv_heads,bs", [(128, 32, 8, 16), (64, 10, 2, 16), (32, 8, 2, 16), (16, 16, 1, 8)])
-def test_shared_prefix_attention_with_peaked_scores_wide_rows_and_unrounded_queries(ops, D, heads, kv_heads, bs):
+def test_shared_prefix_attention_with_peaked_scores_wide_rows_and_unrounded_queries(ops, D, heads, kv_heads, bs, hints):
     # queries three times wider than N(0,1), not representable in fp16: row maxima keep growing behind the first tile
     c = prefix_case(3, D, heads, kv_heads, bs, [(1500, [1, 40, 333]), (260, [600, 2])], peaked=3.0, q_pad=20, o_pad=24, dtype_q=np.float32)
-    check_prefix(c, run_prefix(ops, c), 7.0)
+    check_prefix(c, run_prefix(ops, c, hints), 7.0)
+    if hints:
+        check_prefix(c, run_prefix(ops, padded(c)), 7.0)
 
 
 @pytest.mark.parametrize("hints", [(1, 1), (100000, 100000), (1 << 30, 0)])
@@ -372,30 +394,33 @@ def test_shared_prefix_attention_agrees_with_decode_attention(ops, D, heads, kv_
     assert np.abs(got[c["tokens"]] - want).max() <= 4 * (H16 + 2.0 ** -15) * np.abs(c["v"][~np.isnan(c["v"])].astype(np.float32)).max()
 
 
+@pytest.mark.parametrize("hints", [None, SHARED])
 @pytest.mark.parametrize("D,bs", [(128, 16), (32, 8)])
-def test_shared_prefix_attention_of_a_padded_batch(ops, D, bs):
+def test_shared_prefix_attention_of_a_padded_batch(ops, D, bs, hints):
     # entries before the first group and behind the last are padding, whatever they name
     c = prefix_case(12, D, 8, 2, bs, [(300, [5, 40]), (17, [1, 2, 3])])
     c["tokens"] = np.concatenate([[c["tokens"][1], -1], c["tokens"], [c["tokens"][0]] * 3]).astype(np.int32)
     c["off"] = c["off"] + 2
-    out = run_prefix(ops, c)
+    out = run_prefix(ops, c, hints)
     c["tokens"], c["off"] = c["tokens"][2:-3], c["off"] - 2
     check_prefix(c, out, 7.0)
 
 
-def test_shared_prefix_attention_of_the_same_row_twice(ops):
+@pytest.mark.parametrize("hints", [None, SHARED])
+def test_shared_prefix_attention_of_the_same_row_twice(ops, hints):
     c = prefix_case(13, 64, 8, 2, 16, [(300, [5, 40, 7])])
-    want = run_prefix(ops, c)
+    want = run_prefix(ops, c, hints)
     c["tokens"], c["off"] = np.concatenate([c["tokens"], c["tokens"][:1]]), np.asarray([0, 4], np.int32)
-    assert np.array_equal(run_prefix(ops, c), want)  # one group: either result has the same bits
+    assert np.array_equal(run_prefix(ops, c, hints), want)  # one group: either result has the same bits
 
 
-def test_shared_prefix_attention_scratch_may_hold_anything(ops):
+@pytest.mark.parametrize("hints", [(3000, 30), SHARED])
+def test_shared_prefix_attention_scratch_may_hold_anything(ops, hints):
     c = prefix_case(9, 128, 8, 2, 16, [(3000, [1, 30]), (0, [9]), (100, [4])])
     shape = ops.attn_shape(8, 2, 128, 16)
-    need = ops.shared_prefix_scratch_bytes(shape, 4, 3, c["max_prefix"], c["max_suffix"])
+    need = ops.shared_prefix_scratch_bytes(shape, 4, 3, *hints)
     scratch = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")  # NaN in every word
-    check_prefix(c, run_prefix(ops, c, scratch=scratch[:need]), 7.0)
+    check_prefix(c, run_prefix(ops, c, hints, scratch=scratch[:need]), 7.0)
     assert torch.all(scratch[need:] == 255)
 
 
@@ -413,7 +438,8 @@ def test_page_offsets_past_32_bits(ops, D):
         pool[shift:] = dev(c[name])
         pools.append(pool)
     c["tables"] = (c["tables"] + shift).astype(np.int32)
-    check_prefix(c, run_prefix(ops, c, pools=pools), 7.0)
+    for hints in (None, SHARED):
+        check_prefix(c, run_prefix(ops, c, hints, pools=pools), 7.0)
     qkv = torch.randn(1, (heads + 2 * kv_heads) * D, device="cuda")
     meta = ops.TokenMeta.from_host([3], [0], [0], [nb - 1])
     ops.qkv_norm_post(qkv, None, None, None, 1e-6, torch.ones(D // 2, device="cuda"), meta, qkv, *pools, heads, kv_heads, D, bs)
@@ -577,8 +603,8 @@ class Step:
     """One layer's attention and the sampler of a decode step: 12 requests behind two prompts, one slot of
     the batch unused, under penalties and a grammar; every buffer stays where it is between steps."""
 
-    def __init__(self, ops, seed):
-        self.ops = ops
+    def __init__(self, ops, seed, lengths):
+        self.ops, self.lengths = ops, lengths
         rng = np.random.Generator(np.random.PCG64(seed))
         self.heads, self.kv_heads, self.D, self.bs, self.V = 16, 4, 64, 16, 2000
         self.c = c = prefix_case(seed, self.D, self.heads, self.kv_heads, self.bs,
@@ -610,13 +636,13 @@ class Step:
         self.logits = torch.zeros((T, self.V), device="cuda")
         self.picked = torch.full((T,), -1, dtype=torch.int32, device="cuda")
         self.sampling = torch.zeros((T, 32), dtype=torch.uint8, device="cuda")  # temperature 0
-        self.scratch = torch.empty(ops.shared_prefix_scratch_bytes(self.shape, T, 3, 333, 77), dtype=torch.uint8, device="cuda")
+        self.scratch = torch.empty(ops.shared_prefix_scratch_bytes(self.shape, T, 3, *lengths), dtype=torch.uint8, device="cuda")
 
     def run(self):
         g, o = self.g, self.ops
         o.qkv_norm_post(g["qkv"], None, g["qn"], g["kn"], 1e-5, g["inv"], self.meta, self.q, self.k, self.v, self.heads, self.kv_heads,
                         self.D, self.bs)
-        o.shared_prefix_attention(self.shape, self.q, self.meta, self.tokens, self.off, self.lens, 333, 77, self.k, self.v, self.out,
+        o.shared_prefix_attention(self.shape, self.q, self.meta, self.tokens, self.off, self.lens, *self.lengths, self.k, self.v, self.out,
                                   self.scratch)
         torch.mm(self.out.float(), g["head"].t(), out=self.logits)
         o.adjust_logits(self.logits, self.logits, g["pen"], g["history"], g["history_len"], g["prompt_len"], mask=g["mask"])
@@ -645,15 +671,20 @@ class Step:
         assert self.picked.cpu().tolist() == [oracle.argmax(r) for r in got]
 
 
-def test_a_decode_step_of_all_three_operators(ops):
-    s = Step(ops, 21)
+LENGTHS = [(333, 77), SHARED]
+
+
+@pytest.mark.parametrize("lengths", LENGTHS)
+def test_a_decode_step_of_all_three_operators(ops, lengths):
+    s = Step(ops, 21, lengths)
     s.run()
     torch.cuda.synchronize()
     s.check()
 
 
-def test_a_decode_step_replayed_as_a_graph_follows_its_inputs(ops):
-    s = Step(ops, 22)
+@pytest.mark.parametrize("lengths", LENGTHS)
+def test_a_decode_step_replayed_as_a_graph_follows_its_inputs(ops, lengths):
+    s = Step(ops, 22, lengths)
     s.run()  # attributes are set once per device
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -672,8 +703,9 @@ def test_a_decode_step_replayed_as_a_graph_follows_its_inputs(ops):
             assert torch.equal(a, b)
 
 
-def test_two_decode_steps_at_once_on_two_streams(ops):
-    steps = [Step(ops, 23), Step(ops, 24)]
+@pytest.mark.parametrize("lengths", LENGTHS)
+def test_two_decode_steps_at_once_on_two_streams(ops, lengths):
+    steps = [Step(ops, 23, lengths), Step(ops, 24, lengths)]
     streams = [torch.cuda.Stream() for _ in steps]
     torch.cuda.synchronize()
     for _ in range(20):
