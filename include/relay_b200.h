@@ -400,7 +400,8 @@ int rb200_decode_attention_static(const rb200_attn_shape* s, const float* q, con
  *    decide how the work is split over the GPU; other lengths on the device give the same results up to
  *    rounding. max_prefix 0: nothing is read as shared.
  *  - scratch (rb200_shared_prefix_scratch_bytes, 16-byte aligned, no initial state) holds the
- *    partial results of this call: calls that may overlap need one each.
+ *    partial results of this call: calls that may overlap need one each. A batch that is done in
+ *    one kernel needs 0 bytes; scratch may then be NULL.
  *  - The first call on a device allocates a status word (rb200_gemm_status): make it outside stream
  *    capture.
  * head_dim 16, 32, 64 or 128, at most 16 query heads per KV head; q finite in fp16 (up to 65504) and

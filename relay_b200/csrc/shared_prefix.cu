@@ -709,16 +709,18 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
              part, out, s.heads, s.o_stride);
 }
 
-// Room for a partial of the shared keys where there may be some, whatever the plan.
-size_t scratch_of(const AttnShape& s, int n_decode, int max_prefix, const Plan& p) {
-  return static_cast<size_t>(n_decode) * s.heads * (std::max(p.parts, max_prefix > 0 ? 1 : 0) + p.slices) * (s.D + 2) * sizeof(float);
+// The own keys' partials stay in the CTA where it finishes.
+int partials_of(const Plan& p) { return p.parts + (p.finish ? 0 : p.slices); }
+
+size_t scratch_of(const AttnShape& s, int n_decode, const Plan& p) {
+  return static_cast<size_t>(n_decode) * s.heads * partials_of(p) * (s.D + 2) * sizeof(float);
 }
 
 }  // namespace
 
 size_t shared_prefix_scratch_bytes(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int max_suffix) {
   if (n_decode <= 0 || n_groups <= 0) return 0;
-  return scratch_of(s, n_decode, max_prefix, plan_of(s, n_decode, n_groups, max_prefix, max_suffix));
+  return scratch_of(s, n_decode, plan_of(s, n_decode, n_groups, max_prefix, max_suffix));
 }
 
 void launch_shared_prefix_attention(const AttnShape& s, const float* q, const TokenMeta& m, const int* decode_tokens, int n_decode,
@@ -727,11 +729,14 @@ void launch_shared_prefix_attention(const AttnShape& s, const float* q, const To
                                     cudaStream_t st) {
   if (n_decode == 0) return;
   const Plan plan = plan_of(s, n_decode, n_groups, max_prefix, max_suffix);
-  RB_REQUIRE(scratch_bytes >= scratch_of(s, n_decode, max_prefix, plan), "shared prefix attention: scratch too small");
+  const size_t need = scratch_of(s, n_decode, plan);
+  RB_REQUIRE(scratch != nullptr || need == 0, "shared prefix attention: null scratch");
+  RB_REQUIRE(scratch_bytes >= need, "shared prefix attention: scratch too small");
+  if (umma_prefix_usable(s)) umma_status_word();  // allocated by the first call, whichever kernels that one takes
   const Groups gr{decode_tokens, group_off, plan.parts > 0 ? prefix_len : nullptr, n_decode, n_groups};
   Partials part;
   part.parts = plan.parts;
-  part.total = plan.parts + plan.slices;
+  part.total = partials_of(plan);
   part.o = scratch;
   part.ml = scratch + static_cast<size_t>(n_decode) * s.heads * part.total * s.D;
   switch (s.D) {
@@ -776,7 +781,7 @@ int rb200_shared_prefix_attention(const rb200_attn_shape* s, const float* q, con
     RB_REQUIRE(static_cast<long long>(n_decode) * sh.heads <= 0x7fffffff, "shared prefix attention: bad batch (too many entries)");
     if (n_decode == 0 || n_groups == 0) return 0;  // every entry is padding
     RB_REQUIRE(q && m && m->pos && m->seq && m->table_off && m->tables && decode_tokens && group_off && prefix_len && k_pool &&
-                   v_pool && scratch && out,
+                   v_pool && out,
                "shared prefix attention: null argument");
     for (const void* p : {static_cast<const void*>(q), k_pool, v_pool, static_cast<const void*>(scratch), static_cast<const void*>(out)})
       RB_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "shared prefix attention: q, the pools, scratch and out must be 16-byte aligned");

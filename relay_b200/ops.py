@@ -94,7 +94,7 @@ def decode_attention_static(shape: CAttnShape, q, meta: TokenMeta, decode_tokens
 def _here(op: str, name: str, t: torch.Tensor) -> int:
     """The current CUDA device, which an operator's tensors have to be on; `t` is the first of them."""
     here = t.get_device()
-    if here < 0 or here != torch.cuda.current_device():
+    if here < 0 or here != torch._C._cuda_getDevice():
         raise ValueError(f"{op}: {name} must be on the current CUDA device, not on {t.device}")
     return here
 
@@ -177,11 +177,12 @@ def shared_prefix_attention(shape: CAttnShape, q: torch.Tensor, meta: TokenMeta,
         raise ValueError(f"{op}: out must have the batch's rows, {shape.o_stride} values apart")
     L, sh, m = _lib.lib(), C.byref(shape), meta.c()
     if scratch is None:
-        scratch = torch.empty(max(L.rb200_shared_prefix_scratch_bytes(sh, n, n_groups, max_prefix, max_suffix), 16), dtype=torch.uint8,
-                              device=q.device)
+        need = L.rb200_shared_prefix_scratch_bytes(sh, n, n_groups, max_prefix, max_suffix)
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _lib.check(L.rb200_shared_prefix_attention(
         sh, q.data_ptr(), C.byref(m), decode_tokens.data_ptr(), n, group_off.data_ptr(), prefix_len.data_ptr(), n_groups, max_prefix,
-        max_suffix, k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), out.data_ptr(), _raw_stream(here)))
+        max_suffix, k_pool.data_ptr(), v_pool.data_ptr(), _ptr(scratch), 0 if scratch is None else scratch.numel(), out.data_ptr(),
+        _raw_stream(here)))
     return out
 
 

@@ -1,6 +1,10 @@
 """The decode-step operators around a shared prompt (qkv_norm_post, shared_prefix_attention,
 adjust_logits) against their definitions in float64, at the sizes, masks and layouts where they can
 go wrong, and a run of them together as a step uses them."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -422,6 +426,33 @@ def test_shared_prefix_attention_scratch_may_hold_anything(ops, hints):
     scratch = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")  # NaN in every word
     check_prefix(c, run_prefix(ops, c, hints, scratch=scratch[:need]), 7.0)
     assert torch.all(scratch[need:] == 255)
+
+
+CAPTURE_AFTER_A_SMALL_CALL = """
+import torch
+from relay_b200 import ops
+i32 = dict(dtype=torch.int32, device="cuda")
+shape = ops.attn_shape(8, 2, 64, 16)
+pool = torch.randn(40, 2, 16, 64, device="cuda").half()
+q = torch.randn(1, 12 * 64, device="cuda")
+meta = ops.TokenMeta(torch.tensor([599], **i32), torch.tensor([0], **i32), torch.tensor([0], **i32), torch.arange(40, **i32))
+args = shape, q, meta, torch.tensor([0], **i32), torch.tensor([0, 1], **i32), torch.tensor([590], **i32)
+outs = [torch.zeros(1, 512, dtype=torch.float16, device="cuda") for _ in range(2)]
+ops.shared_prefix_attention(*args, 590, 10, pool, pool, outs[0])
+scratch = torch.empty(ops.shared_prefix_scratch_bytes(shape, 1, 1, 1 << 20, 0), dtype=torch.uint8, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.shared_prefix_attention(*args, 1 << 20, 0, pool, pool, outs[1], scratch)
+graph.replay()
+torch.cuda.synchronize()
+assert (outs[0].float() - outs[1].float()).abs().max() <= (2.0 ** -9 + 2.0 ** -14) * pool.float().abs().max()
+"""
+
+
+def test_shared_prefix_attention_captured_after_a_small_call(ops):
+    # in a process of its own: the small call is the device's first, and takes other kernels than the captured one
+    subprocess.run([sys.executable, "-c", CAPTURE_AFTER_A_SMALL_CALL], check=True, timeout=300,
+                   cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 
 @pytest.mark.parametrize("D", [128, 32])

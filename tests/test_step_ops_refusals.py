@@ -67,9 +67,9 @@ def prefix(shape=(32, 8, 128, 16, 6144, 4096), **kw):
     (dict(shape=(32, 8, 128, 16, 6146, 4096)), "multiple"), (dict(shape=(32, 8, 128, 16, 6144, 4100)), "multiple"),
     (dict(n=-1), "bad batch"), (dict(n=1 << 27), "bad batch"), (dict(groups=-1), "bad batch"), (dict(max_prefix=-1), "bad batch"), (dict(max_suffix=-1), "bad batch"),
     (dict(q=None), "null"), (dict(meta=None), "null"), (dict(tokens=None), "null"), (dict(off=None), "null"), (dict(lens=None), "null"),
-    (dict(k=None), "null"), (dict(v=None), "null"), (dict(scratch=None), "null"), (dict(out=None), "null"),
+    (dict(k=None), "null"), (dict(v=None), "null"), (dict(scratch=None, max_prefix=100000), "null scratch"), (dict(out=None), "null"),
     (dict(q=C.c_void_p(4104)), "aligned"), (dict(k=C.c_void_p(4098)), "aligned"), (dict(out=C.c_void_p(4104)), "aligned"),
-    (dict(scratch=C.c_void_p(4100)), "aligned"), (dict(scratch_bytes=1000), "scratch too small"),
+    (dict(scratch=C.c_void_p(4100)), "aligned"), (dict(scratch_bytes=1000, max_prefix=100000), "scratch too small"),
 ])
 def test_shared_prefix_attention_refuses(kw, text):
     refused(prefix(**kw), text)
@@ -83,8 +83,8 @@ def test_shared_prefix_scratch_is_host_computable():
     L = _lib.lib()
     sh = _lib.CAttnShape(32, 8, 128, 16, 6144, 4096)
     per = 4 * 32 * 130 * 4  # one slice of four tokens: (D + 2) floats per (token, head)
-    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 100, 100) == 2 * per  # of the shared keys and of the own ones
-    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 0, 100) == per
+    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 100, 100) == 0  # one kernel
+    assert L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, 0, 100) == 0
     for lens in ((100000, 100), (100, 100000)):
         many = L.rb200_shared_prefix_scratch_bytes(C.byref(sh), 4, 1, *lens)
         assert many > 2 * per and many % per == 0
