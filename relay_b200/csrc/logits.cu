@@ -1,12 +1,12 @@
 // What a request asks of its logits ahead of the sampler: penalties for tokens that occur in its
 // history, biases, and a grammar's mask, in one pass over the row.
 //
-// A CTA owns a segment of one row's vocabulary. What the mask leaves of its logits goes to registers (a vector
-// of four that the mask takes whole is not read) while the history's tokens of the segment are counted in
-// shared memory: integer atomics, so the counts do not depend on their order. Then each value is adjusted
-// and stored. The few biases follow as a correction of what was stored, with the counters' memory
-// now holding the last entry of each biased token. At most 8 bytes per logit move, plus one bit of mask:
-// the kernel is bound by memory, and by latency for a few rows.
+// A CTA owns a segment of one row's vocabulary. It counts the history's tokens of the segment in shared memory
+// (integer atomics, so the counts do not depend on their order) and reads which logits the mask leaves; then each
+// of these is read, adjusted and stored (a vector of four that the mask takes whole is not read), while
+// other CTAs of the SM are at their counts. The few biases follow as a correction of what was stored, with the
+// counters' memory now holding the last entry of each biased token. At most 8 bytes per logit move, plus one
+// bit of mask: the kernel is bound by memory, and by latency for a few rows.
 #include <climits>
 
 #include "kernels.h"
@@ -16,6 +16,7 @@ namespace rb200 {
 namespace {
 
 constexpr int kLgThreads = 512;
+
 constexpr uint32_t kSeen = 0x80000000u;  // the token occurs; the bits below count the generated ones
 
 struct LogitArgs {
@@ -41,7 +42,7 @@ __device__ __forceinline__ bool allowed(const uint32_t* mask, int v) { return ma
 // NV vectors of 4 logits per thread: a segment of 4 kLgThreads NV tokens. Segments are cut on the 16-byte grid
 // of the row's memory, so the row's first `shift` (0..3) places of segment 0 lie ahead of the row.
 template <int NV>
-__global__ void __launch_bounds__(kLgThreads, 1024 / kLgThreads)
+__global__ void __launch_bounds__(kLgThreads, 3)
 adjust_logits_kernel(const LogitArgs a) {
   constexpr int kSegment = kLgThreads * 4 * NV;
   extern __shared__ uint32_t count[];  // [kSegment]
@@ -69,40 +70,23 @@ adjust_logits_kernel(const LogitArgs a) {
   }
   if (a.bias_ids) biases = a.bias_len[r];
 
-  // Which values are in the row and pass the mask, four bits for each vector, and the values. A segment that lies
-  // inside the row on the mask's own grid needs no look at the row's ends.
+  // Which values are in the row and pass the mask, four bits for each vector. A segment that lies inside the row on the
+  // mask's own grid needs no look at the row's ends.
   const bool inside = shift == 0 && v0 + kSegment <= V;
   uint32_t keep = 0;
-  float4 val[NV];
   if (inside) {
     uint32_t word[NV];
 #pragma unroll
     for (int n = 0; n < NV; ++n) word[n] = mask ? mask[(v0 >> 5) + n * (kLgThreads / 8) + (tid >> 3)] : 0xffffffffu;
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const uint32_t bits = (word[n] >> ((tid & 7) * 4)) & 15u;
-      keep |= bits << (4 * n);
-      val[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (bits) val[n] = *reinterpret_cast<const float4*>(x + v0 + (n * kLgThreads + tid) * 4);
-    }
+    for (int n = 0; n < NV; ++n) keep |= (word[n] >> ((tid & 7) * 4) & 15u) << (4 * n);
   } else {
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int v = v0 + (n * kLgThreads + tid) * 4;
-      uint32_t bits = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (v + e >= 0 && v + e < V && allowed(mask, v + e)) bits |= 1u << e;
-      keep |= bits << (4 * n);
-      val[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (v >= 0 && v + 4 <= V) {
-        if (bits) val[n] = *reinterpret_cast<const float4*>(x + v);
-      } else {
-        if (bits & 1u) val[n].x = x[v];
-        if (bits & 2u) val[n].y = x[v + 1];
-        if (bits & 4u) val[n].z = x[v + 2];
-        if (bits & 8u) val[n].w = x[v + 3];
-      }
+        if (v + e >= 0 && v + e < V && allowed(mask, v + e)) keep |= 1u << (4 * n + e);
     }
   }
 
@@ -137,29 +121,50 @@ adjust_logits_kernel(const LogitArgs a) {
     __syncthreads();
   }
 
+  // The values, B vectors of a thread at a time: 53 us for 256 rows of 128256 logits. (All of them on their way ahead of
+  // the count leave registers for two CTAs to an SM instead of three: 63. The first B ahead of it spill: 69.)
   const float inverse = 1.0f / pen.repetition;
+  constexpr int B = NV < 4 ? NV : 4;
 #pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int at = (n * kLgThreads + tid) * 4, v = v0 + at;
-    const uint32_t bits = keep >> (4 * n) & 15u;
-    bool changed = !in_place || bits != 15u;
-    if (counted) {
-      const uint4 c = *reinterpret_cast<const uint4*>(count + at);
-      if (c.x | c.y | c.z | c.w) {
-        changed = true;
-        val[n].x = adjusted(val[n].x, c.x, pen, inverse), val[n].y = adjusted(val[n].y, c.y, pen, inverse);
-        val[n].z = adjusted(val[n].z, c.z, pen, inverse), val[n].w = adjusted(val[n].w, c.w, pen, inverse);
+  for (int n0 = 0; n0 < NV; n0 += B) {
+    float4 val[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int n = n0 + j, v = v0 + (n * kLgThreads + tid) * 4;
+      const uint32_t bits = keep >> (4 * n) & 15u;
+      val[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (inside || (v >= 0 && v + 4 <= V)) {
+        if (bits) val[j] = *reinterpret_cast<const float4*>(x + v);
+      } else {
+        if (bits & 1u) val[j].x = x[v];
+        if (bits & 2u) val[j].y = x[v + 1];
+        if (bits & 4u) val[j].z = x[v + 2];
+        if (bits & 8u) val[j].w = x[v + 3];
       }
     }
-    if (!changed) continue;
-    const float y[4] = {bits & 1u ? val[n].x : -INFINITY, bits & 2u ? val[n].y : -INFINITY, bits & 4u ? val[n].z : -INFINITY,
-                        bits & 8u ? val[n].w : -INFINITY};
-    if (same_grid && (inside || (v >= 0 && v + 4 <= V))) {
-      *reinterpret_cast<float4*>(o + v) = make_float4(y[0], y[1], y[2], y[3]);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (v + e >= 0 && v + e < V) o[v + e] = y[e];
+    for (int j = 0; j < B; ++j) {
+      const int n = n0 + j, at = (n * kLgThreads + tid) * 4, v = v0 + at;
+      const uint32_t bits = keep >> (4 * n) & 15u;
+      bool changed = !in_place || bits != 15u;
+      if (counted) {
+        const uint4 c = *reinterpret_cast<const uint4*>(count + at);
+        if (c.x | c.y | c.z | c.w) {
+          changed = true;
+          val[j].x = adjusted(val[j].x, c.x, pen, inverse), val[j].y = adjusted(val[j].y, c.y, pen, inverse);
+          val[j].z = adjusted(val[j].z, c.z, pen, inverse), val[j].w = adjusted(val[j].w, c.w, pen, inverse);
+        }
+      }
+      if (!changed) continue;
+      const float y[4] = {bits & 1u ? val[j].x : -INFINITY, bits & 2u ? val[j].y : -INFINITY, bits & 4u ? val[j].z : -INFINITY,
+                          bits & 8u ? val[j].w : -INFINITY};
+      if (same_grid && (inside || (v >= 0 && v + 4 <= V))) {
+        *reinterpret_cast<float4*>(o + v) = make_float4(y[0], y[1], y[2], y[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v + e >= 0 && v + e < V) o[v + e] = y[e];
+      }
     }
   }
 
@@ -206,12 +211,16 @@ void launch_adjust_logits(const float* logits, int ld_logits, float* out, int ld
   if (R == 0) return;
   const LogitArgs a{logits, out, penalties, history, history_len, prompt_len, bias_ids, bias_values, bias_len, mask,
                     ld_logits, ld_out, V, ld_history, ld_bias, ld_mask};
-  // Every segment reads its row's whole history, so segments are as long as leaves two CTAs for every SM: 256 rows of
-  // 128256 logits with 4116 tokens each take 63 us in segments of 16384, 68, 112 and 179 in 8192, 4096 and 2048.
-  // (Clusters that read a history once and count in the owner's shared memory: 119 us.)
-  const long long places = V + 3LL, want = 2LL * sm_count();
-  if (R * (places / (kLgThreads * 32)) >= want) launch_segments<8>(a, R, st);
-  else if (R * (places / (kLgThreads * 16)) >= want) launch_segments<4>(a, R, st);
+  // Every segment reads its row's whole history, so segments are as long as leaves the GPU busy: three CTAs for every SM
+  // in segments of 16384, two in 8192, one in 4096, otherwise 2048. Measured at 128256 logits and histories of 8192:
+  // 256 rows 58, 70, 99 and 153 us in 16384, 8192, 4096 and 2048; 32 rows 11.8 in 8192, 13.9 in 4096; 16 rows 8.7 and 8.8;
+  // 8 rows 6.8 in 4096, 7.5 in 2048; one row with 800 tokens 3.9 and 3.5.
+  // (Clusters that read a history once and count in the owner's shared memory: 119 us for 256 rows; a list of the counted
+  // tokens, whose values alone are adjusted once the others are stored: 77, against 53 with histories of 40 - 8192.)
+  const long long places = V + 3LL, sms = sm_count();
+  if (R * (places / (kLgThreads * 32)) >= 3 * sms) launch_segments<8>(a, R, st);
+  else if (R * (places / (kLgThreads * 16)) >= 2 * sms) launch_segments<4>(a, R, st);
+  else if (R * (places / (kLgThreads * 8)) >= sms) launch_segments<2>(a, R, st);
   else launch_segments<1>(a, R, st);
 }
 

@@ -533,11 +533,15 @@ LOGIT_CASES = [
     (3, 5000, 0, 0, True),
     (3, 5000, 12, 0, False),
     (2, 300000, 50000, 1000, True),
-    # batches whose segments are long: 4 of 8192 tokens; clusters of 8, 2 x 5 and 2 segments of 16384
+    # batches whose segments are long: of 4096, of 8192 and of 16384 tokens
+    (6, 128256, 900, 3, True),
+    (5, 151937, 900, 0, False),
     (100, 33000, 700, 3, True),
     (48, 128256, 3000, 16, True),
     (40, 151937, 5000, 0, False),
     (300, 20000, 60, 2, True),
+    (64, 128256, 3000, 16, True),
+    (64, 151937, 300, 40, True),
 ]
 
 
