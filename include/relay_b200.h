@@ -385,9 +385,11 @@ int rb200_decode_attention_static(const rb200_attn_shape* s, const float* q, con
  * same keys (samples of one prompt, questions about one document): entries group_off[g] ..
  * group_off[g + 1] - 1 of decode_tokens are a group whose first prefix_len[g] keys are the same,
  * so these are read once for the group, through the block table of its first entry, and each
- * entry's other keys through its own table. The result is that of rb200_decode_attention on
- * the same batch, up to rounding. q, m, decode_tokens, the pools and out are as there; group_off
- * (n_groups + 1 entries, ascending) and prefix_len (n_groups) are device arrays.
+ * entry's other keys through its own table; a small batch behind a short prefix reads all keys of
+ * an entry through its own table, which is therefore complete. The result is that of
+ * rb200_decode_attention on the same batch, up to rounding. q, m, decode_tokens, the pools and
+ * out are as there; group_off (n_groups + 1 entries, ascending) and prefix_len (n_groups) are
+ * device arrays.
  *  - A group counts min(prefix_len[g], context of its first entry) keys as shared; 0 is allowed,
  *    and so is any length, also one that ends inside a block (the blocks up to there have to hold
  *    the same keys, they need not be the same blocks). An entry with a shorter context than its

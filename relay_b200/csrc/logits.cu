@@ -121,7 +121,7 @@ adjust_logits_kernel(const LogitArgs a) {
     __syncthreads();
   }
 
-  // The values, B vectors of a thread at a time: 53 us for 256 rows of 128256 logits. (All of them on their way ahead of
+  // The values, B vectors of a thread at a time: 51 us for 256 rows of 128256 logits. (All of them on their way ahead of
   // the count leave registers for two CTAs to an SM instead of three: 63. The first B ahead of it spill: 69.)
   const float inverse = 1.0f / pen.repetition;
   constexpr int B = NV < 4 ? NV : 4;
@@ -147,7 +147,7 @@ adjust_logits_kernel(const LogitArgs a) {
       const int n = n0 + j, at = (n * kLgThreads + tid) * 4, v = v0 + at;
       const uint32_t bits = keep >> (4 * n) & 15u;
       bool changed = !in_place || bits != 15u;
-      if (counted) {
+      if (counted && bits) {
         const uint4 c = *reinterpret_cast<const uint4*>(count + at);
         if (c.x | c.y | c.z | c.w) {
           changed = true;
@@ -213,10 +213,10 @@ void launch_adjust_logits(const float* logits, int ld_logits, float* out, int ld
                     ld_logits, ld_out, V, ld_history, ld_bias, ld_mask};
   // Every segment reads its row's whole history, so segments are as long as leaves the GPU busy: three CTAs for every SM
   // in segments of 16384, two in 8192, one in 4096, otherwise 2048. Measured at 128256 logits and histories of 8192:
-  // 256 rows 58, 70, 99 and 153 us in 16384, 8192, 4096 and 2048; 32 rows 11.8 in 8192, 13.9 in 4096; 16 rows 8.7 and 8.8;
+  // 256 rows 57, 70, 99 and 153 us in 16384, 8192, 4096 and 2048; 32 rows 11.8 in 8192, 13.9 in 4096; 16 rows 8.7 and 8.8;
   // 8 rows 6.8 in 4096, 7.5 in 2048; one row with 800 tokens 3.9 and 3.5.
   // (Clusters that read a history once and count in the owner's shared memory: 119 us for 256 rows; a list of the counted
-  // tokens, whose values alone are adjusted once the others are stored: 77, against 53 with histories of 40 - 8192.)
+  // tokens, whose values alone are adjusted once the others are stored: 77, against 51 with histories of 40 - 8192.)
   const long long places = V + 3LL, sms = sm_count();
   if (R * (places / (kLgThreads * 32)) >= 3 * sms) launch_segments<8>(a, R, st);
   else if (R * (places / (kLgThreads * 16)) >= 2 * sms) launch_segments<4>(a, R, st);

@@ -15,13 +15,13 @@ namespace rb200 {
 
 namespace {
 
-constexpr int kQnWarps = 8;   // of qkv_norm_post_kernel
+constexpr int kQnWarps = 8;       // of qkv_norm_post_kernel
 constexpr int kQnRounds = 4;      // rounds of a warp in flight in qkv_norm_vec_kernel
 constexpr int kQnPairRounds = 2;  // and in qkv_norm_pair_kernel
 
-// cos and sin of pos * inv_freq. The product is exact in float64 and reduced there, in units of pi: its float32
-// rounding alone would be off by 4e-3 rad at position 131072. What is left, at most 1, rounds to float32
-// within 2^-24 of itself.
+// cos and sin of pos * inv_freq. The product is taken in float64 (exact below position 2^29) and reduced there, in
+// units of pi: its float32 rounding alone would be off by 4e-3 rad at position 131072. What is left, at most 1,
+// rounds to float32 within 2^-24 of itself.
 __device__ __forceinline__ void rotation(int pos, float inv_freq, float& c, float& s) {
   constexpr double kInvTwoPi = 0.15915494309189533577;
   const double turns = static_cast<double>(pos) * static_cast<double>(inv_freq) * kInvTwoPi;
