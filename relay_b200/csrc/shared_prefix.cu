@@ -591,8 +591,8 @@ struct Plan {
 //  * a CTA of the prefix kernel takes kTileUs for every 128 keys and kStartUs besides, and the join kJoinUs; the own keys
 //    (six tenths of the most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel
 //    leaves free get kBytesPerSmUs each until it ends. Measured at 32 + 2 x 8 heads of 128: 256 tokens behind 8192 keys
-//    with 128 - 640 of their own, 108 us in one slice (64 CTAs beside the own keys) and 120 in two, which fill the
-//    GPU; 32 tokens behind 4096 with 64 - 512: 25, 22, 26 and 27 us in 4, 8, 11 and 16 slices;
+//    with 128 - 640 of their own, 105 us in one slice (64 CTAs beside the own keys) and 117 in two, which fill the
+//    GPU; 32 tokens behind 4096 with 64 - 512: 24, 20.5, 25 and 28 us in 4, 8, 11 and 16 slices;
 //  * the suffix kernel takes kOwnStartUs and for every key of a slice 5 ns and 35 ps a value of the head (blocks that
 //    16 keys do not divide: 2.5 ns more), 0.6 of that in CTAs of eight warps (`wide`), and where there are more CTAs than
 //    SMs eight tenths of it times the CTAs to an SM; slices take kOwnJoinUs more;
