@@ -587,6 +587,13 @@ struct Plan {
   bool finish, wide;
 };
 
+// The own keys' partials stay in the CTA where it finishes.
+int partials_of(const Plan& p) { return p.parts + (p.finish ? 0 : p.slices); }
+
+size_t scratch_of(const AttnShape& s, int n_decode, const Plan& p) {
+  return static_cast<size_t>(n_decode) * s.heads * partials_of(p) * (s.D + 2) * sizeof(float);
+}
+
 // The plan follows from estimates in us:
 //  * a CTA of the prefix kernel takes kTileUs for every 128 keys and kStartUs besides, and the join kJoinUs; the own keys
 //    (six tenths of the most) take their bytes at kBytesPerUs of the whole GPU, of which the SMs that the prefix kernel
@@ -594,18 +601,20 @@ struct Plan {
 //    with 128 - 640 of their own, 105 us in one slice (64 CTAs beside the own keys) and 117 in two, which fill the
 //    GPU; 32 tokens behind 4096 with 64 - 512: 24, 20.5, 25 and 28 us in 4, 8, 11 and 16 slices;
 //  * the suffix kernel takes kOwnStartUs and for every key of a slice 5 ns and 35 ps a value of the head (blocks that
-//    16 keys do not divide: 2.5 ns more), 0.6 of that in CTAs of eight warps (`wide`), and where there are more CTAs than
-//    SMs eight tenths of it times the CTAs to an SM; slices take kOwnJoinUs more;
-//  * a launch behind the first counts kLaunchUs, of the 2.5 us of the caller's time for it that a graph does not spend.
-// Measured over 150 batches of 1 - 48 tokens behind 100 - 3000 keys in five head layouts: all keys as the tokens' own
-// 5.1 us against 10.3 shared at 16 tokens of 8 KV heads of 128 behind 100 keys, 7.8 against 10.8 behind 500, 21 against
-// 14 behind 3000; one token behind 500 keys 6.9 against 8.5 in CTAs of four warps.
+//    16 keys do not divide: 2.5 ns more), 0.6 of that in CTAs of eight warps (`wide`); with x CTAs to an SM 0.65 + x / 2
+//    times as much (heads of 64 and less: 0.65 + 0.35 x). Slices take kOwnJoinUs more;
+//  * a launch behind the first counts kLaunchUs, most of the 2.5 us of the caller's time for it, which a graph does
+//    not spend.
+// Measured over 400 batches of 1 - 512 tokens in 1 - 64 groups behind 64 - 3000 keys in five head layouts, where the plan
+// takes at most 20 % or 2 us longer than the better of both ways: all keys as the tokens' own 5.1 us against 10.3 shared
+// at 16 tokens of 8 KV heads of 128 behind 100 keys, 7.8 against 10.8 behind 500, 21 against 14 behind 3000; one
+// token behind 500 keys 6.9 against 8.5 in CTAs of four warps.
 constexpr double kTileUs = 1.3, kStartUs = 6.0, kJoinUs = 1.5, kBytesPerUs = 5.5e6, kBytesPerSmUs = 4.2e4;
 constexpr double kOwnStartUs = 3.8, kOwnJoinUs = 2.0, kLaunchUs = 2.0;
 
 double own_us(const AttnShape& s, long long pairs, double keys, int slices, bool wide) {
   const double key_us = (0.005 + 35e-6 * s.D + (s.block_size % 16 == 0 ? 0.0 : 0.0025)) * (wide ? 0.6 : 1.0);
-  const double load = 0.8 * static_cast<double>(pairs * slices) / sm_count();
+  const double share = s.D == 128 ? 0.5 : 0.35, load = share * static_cast<double>(pairs * slices) / sm_count() + 0.65;
   return kOwnStartUs + keys / slices * key_us * std::max(1.0, load) + (slices > 1 ? kOwnJoinUs + kLaunchUs : 0.0);
 }
 
@@ -638,18 +647,23 @@ Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int
   p.rows = umma_prefix_usable(s) && static_cast<long long>(n_decode) * (s.heads / s.kv_heads) > 64LL * n_groups ? 128 : 64;
   p.tiles = static_cast<int>(row_tiles(s, n_decode, n_groups, p.rows));
   const long long ctas = static_cast<long long>(p.tiles) * s.kv_heads;
-  const long long slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();  // one CTA of the tcgen05 kernel fits an SM
+  const long long slots = (umma_prefix_usable(s) ? 1LL : 2LL) * sm_count();
   const double suffix_us = 0.6 * 4.0 * max_suffix * s.D * static_cast<double>(pairs) / kBytesPerUs;
+  // The time of n slices with `running` CTAs, and how much of the own keys' time that takes along.
+  auto shared_us = [&](long long running, int n, double tile_us) {
+    return static_cast<double>((running + slots - 1) / slots) * (div_up(div_up(max_prefix, n), kPrefixSlice) * tile_us + kStartUs);
+  };
+  auto beside_us = [&](long long running, double us) {
+    const double idle = std::max<double>(0.0, 1.0 - static_cast<double>(running) / slots) * sm_count();
+    return us * std::min(1.0, idle * kBytesPerSmUs / kBytesPerUs);
+  };
   double least = -1.0, prefix_us = 0.0;
   for (int n = 1; n <= kMostParts && (n == 1 || max_prefix > (n - 1) * 2 * kPrefixSlice); ++n) {
-    const double waves = static_cast<double>((ctas * n + slots - 1) / slots);
-    const double shared_us = waves * (div_up(div_up(max_prefix, n), kPrefixSlice) * kTileUs + kStartUs);
-    const double idle = std::max<double>(0.0, 1.0 - static_cast<double>(ctas * n) / slots) * sm_count();
-    const double beside = shared_us * std::min(1.0, idle * kBytesPerSmUs / kBytesPerUs);
-    const double us = shared_us + std::max(0.0, suffix_us - beside);
+    const double shared = shared_us(ctas * n, n, kTileUs);
+    const double us = shared + std::max(0.0, suffix_us - beside_us(ctas * n, shared));
     if (least < 0.0 || us < least) {
       least = us;
-      prefix_us = shared_us;
+      prefix_us = shared;
       p.parts = n;
     }
   }
@@ -657,7 +671,17 @@ Plan plan_of(const AttnShape& s, int n_decode, int n_groups, int max_prefix, int
   const bool beside = pairs <= 2LL * sm_count() - (umma_prefix_usable(s) ? 2 : 1) * ctas * p.parts;
   p.slices = beside && own_us(s, pairs, max_suffix, 1, false) <= prefix_us ? 1 : most_slices(max_suffix);
   p.finish = beside && p.slices == 1;
-  return alone_us <= least + kJoinUs + (p.finish ? 1 : 2) * kLaunchUs ? alone : p;
+
+  // Both ways against each other, with as many row tiles as groups of one size have. Two CTAs of prefix_mma_kernel on an SM
+  // take 1.6 times as long for their tiles.
+  const long long rows = static_cast<long long>(n_decode) * (s.heads / s.kv_heads);
+  const long long expected = n_groups * static_cast<long long>(div_up(rows, static_cast<long long>(n_groups) * p.rows));
+  const long long running = std::min<long long>(p.tiles, expected) * s.kv_heads * p.parts;
+  prefix_us = shared_us(running, p.parts, umma_prefix_usable(s) || running <= sm_count() ? kTileUs : 1.6 * kTileUs);
+  const double own = std::max(suffix_us, own_us(s, pairs, max_suffix, 1, false));
+  const double behind_us = std::max(0.0, own - beside_us(running, prefix_us));
+  const double join_us = kJoinUs + 2.0 * static_cast<double>(scratch_of(s, n_decode, p)) / kBytesPerUs;
+  return alone_us <= prefix_us + behind_us + join_us + (p.finish ? 1 : 2) * kLaunchUs ? alone : p;
 }
 
 template <int D, bool CONTIG, int NT, int W, int S>
@@ -707,13 +731,6 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
   count_launch();
   launch_pdl(join_kernel<D>, dim3(div_up(static_cast<long long>(gr.n_decode) * s.heads, kJoinWarps)), dim3(kJoinWarps * 32), 0, st, m, gr,
              part, out, s.heads, s.o_stride);
-}
-
-// The own keys' partials stay in the CTA where it finishes.
-int partials_of(const Plan& p) { return p.parts + (p.finish ? 0 : p.slices); }
-
-size_t scratch_of(const AttnShape& s, int n_decode, const Plan& p) {
-  return static_cast<size_t>(n_decode) * s.heads * partials_of(p) * (s.D + 2) * sizeof(float);
 }
 
 }  // namespace
