@@ -604,7 +604,7 @@ void launch_decode_t(const AttnShape& s, const float* q, const TokenMeta& m, con
                      cudaStream_t st, bool cluster_merge) {
   static PerDeviceOnce once;
   auto kernel = decode_split_kernel<D, CONTIG, WIDE>;
-  if (once.first()) raise_smem(kernel, decode_smem_bytes<D>());
+  once.run([&] { raise_smem(kernel, decode_smem_bytes<D>()); });
   RB_REQUIRE(!cluster_merge || parts <= 8, "decode attention: a cluster holds at most 8 slices");
   const float scale_log2e = kLog2e / sqrtf(static_cast<float>(D));
   dim3 grid(n_decode, s.kv_heads, parts);
@@ -651,7 +651,7 @@ void launch_prefill_d(const AttnShape& s, const float* q, const TokenMeta& m, co
                       const __half* kc, const __half* vc, __half* out, cudaStream_t st) {
   static PerDeviceOnce once;
   auto kernel = prefill_flash_kernel<D>;
-  if (once.first()) raise_smem(kernel, prefill_smem_bytes<D>());
+  once.run([&] { raise_smem(kernel, prefill_smem_bytes<D>()); });
   const float scale_log2e = kLog2e / sqrtf(static_cast<float>(D));
   dim3 grid(n_tiles, s.heads);
   count_launch();

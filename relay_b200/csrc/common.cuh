@@ -69,19 +69,24 @@ int sm_count();
 
 // A kernel attribute (cudaFuncSetAttribute) belongs to the device that is current when it is
 // set, so a process that drives several GPUs has to set it once on each. One of these, as a
-// function-local static next to the launch, remembers the devices already done; first() is
-// true once per device (two threads racing on it both set the attribute, which is harmless:
-// the call is idempotent and only ever raises the limit).
+// function-local static next to the launch, remembers the devices already done. A device is done
+// only when `set` has returned: a thread that comes while another is still at it sets the
+// attribute, too (harmless: the call is idempotent and only ever raises the limit) instead of
+// launching without it, and a `set` that throws is tried again by the next call.
 struct PerDeviceOnce {
   static constexpr int kMaxDevices = 64;
   std::atomic<bool> done[kMaxDevices] = {};
-  bool first() {
+  template <class F>
+  void run(F&& set) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
       cudaGetLastError();
-      return true;  // unknown device: set the attribute every time
+      set();  // unknown device: every time
+      return;
     }
-    return !done[dev].exchange(true, std::memory_order_acq_rel);
+    if (done[dev].load(std::memory_order_acquire)) return;
+    set();
+    done[dev].store(true, std::memory_order_release);
   }
 };
 

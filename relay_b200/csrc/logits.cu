@@ -196,8 +196,9 @@ void launch_segments(const LogitArgs& a, int R, cudaStream_t st) {
   constexpr int kSegment = kLgThreads * 4 * NV;
   static PerDeviceOnce once;
   auto kernel = adjust_logits_kernel<NV>;
-  if (once.first())
+  once.run([&] {
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSegment * 4));
+  });
   count_launch();
   launch_pdl(kernel, dim3(div_up(a.V + 3LL, kSegment), R), dim3(kLgThreads), kSegment * 4, st, a);
 }

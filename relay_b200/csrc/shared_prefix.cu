@@ -689,8 +689,9 @@ void launch_suffix(const AttnShape& s, const float* q, const TokenMeta& m, const
                    const Partials& part, __half* out, const Plan& plan, cudaStream_t st) {
   static PerDeviceOnce once;
   auto kernel = suffix_kernel<D, CONTIG, NT, W, S>;
-  if (once.first())
+  once.run([&] {
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(suffix_smem_bytes<D, W, S>())));
+  });
   count_launch();
   const int first = plan.parts == 0, finish = plan.finish;
   launch_pdl(kernel, dim3(gr.n_decode, s.kv_heads, plan.slices), dim3(W * 32), suffix_smem_bytes<D, W, S>(), st, q, m, gr, kc, vc, part,
@@ -707,8 +708,9 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
     } else {
       static PerDeviceOnce once;
       auto kernel = prefix_mma_kernel<D>;
-      if (once.first())
+      once.run([&] {
         RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(prefix_smem_bytes<D>())));
+      });
       count_launch();
       launch_pdl(kernel, dim3(plan.tiles, s.kv_heads, plan.parts), dim3(128), prefix_smem_bytes<D>(), st, q, m, gr, kc, vc, part, s.heads,
                  s.kv_heads, s.block_size, shift_of(s.block_size), s.q_stride, kLog2e / sqrtf(static_cast<float>(D)));

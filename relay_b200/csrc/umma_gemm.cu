@@ -486,8 +486,9 @@ void launch_umma_cfg(const WeightView& W, const __half* x, int ldx, float* y, in
   using S = UmmaSmem<BN, INT8, MT>;
   static PerDeviceOnce once;
   auto kernel = umma_gemm_kernel<BN, INT8, MT>;
-  if (once.first())
+  once.run([&] {
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kTotal)));
+  });
   const CUtensorMap mw = INT8 ? make_map(W.i8, 1, W.N, W.K, W.ld, rows, S::kKB, S::kKB == 128, S::kKB == 64)
                               : make_map(W.f16, 2, W.N, W.K, W.ld, rows, kBlockK, true);
   const CUtensorMap mx = make_map(x, 2, T, W.K, ldx, BN, kBlockK, true);

@@ -454,8 +454,9 @@ void launch_i8_t(const WeightView& W, const int8_t* digits, const float* tscale,
   using S = I8Smem<BN>;
   static PerDeviceOnce once;
   auto kernel = umma_i8_kernel<BN, FUSED>;
-  if (once.first())
+  once.run([&] {
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kTotal)));
+  });
   // Rows per CTA and the K split: the pair that needs the fewest (waves x bytes per CTA), where a
   // CTA's fixed cost (prologue, pipeline fill, epilogue) counts like 48 KB of weights. A cluster
   // needs its CTAs on SMs of one GPC at the same time, so fewer clusters than SMs / size are

@@ -425,8 +425,9 @@ void launch_umma_prefill_d(const AttnShape& s, const float* q, const TokenMeta& 
   using S = PfSmem<D>;
   static PerDeviceOnce once;
   auto kernel = umma_prefill_kernel<D>;
-  if (once.first())
+  once.run([&] {
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kTotal)));
+  });
   // The layer's pool as rows of D halves, box = one 16-key page x 64 dims. With the pool's real
   // row count a page outside it reads as zeros; callers that do not know it get a bound that only
   // limits the coordinates (the kernel never asks for a row the block table does not name).

@@ -415,8 +415,9 @@ void launch_d(const AttnShape& s, const float* q, const TokenMeta& m, const Grou
   using S = Smem<D, ROWS>;
   static PerDeviceOnce once;
   auto kernel = umma_prefix_kernel<D, ROWS>;
-  if (once.first())
+  once.run([&] {
     RB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kTotal)));
+  });
   // The pool as rows of D halves, box = one 16-key page x 64 dims. The row count only limits the
   // coordinates: the kernel asks for no row that the block table does not name.
   const CUtensorMap mk = make_map(kc, 2, 1LL << 31, D, D, 16, 64, true);
