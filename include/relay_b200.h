@@ -478,7 +478,7 @@ int rb200_qkv_post(float* qkv, const float* bias, const float* inv_freq, const r
  * rot_dim values (pairs (i, i + rot_dim / 2), the others pass; inv_freq: [rot_dim / 2]), q to q_out
  * and k and v as fp16 to the token's slot of the paged pools. The angle pos * inv_freq is taken in
  * 64 bits, so it stays exact at far positions. qkv rows are qkv_stride floats apart, rows of q_out
- * q_stride; q_out may be qkv itself with the same stride (q in place), any other overlap is
+ * q_stride; q_out may be qkv itself with the same stride (q in place; any stride for one token), any other overlap is
  * not allowed. Of qkv only that q part is written. A token with seq < 0 or pos < 0 is padding:
  * its row of q_out stays as it was and nothing is appended. Two tokens of one call must not share a slot. head_dim even and at
  * most 256; rot_dim even, 0 (inv_freq may be NULL) to head_dim. bias may be NULL. */

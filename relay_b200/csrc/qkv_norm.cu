@@ -384,7 +384,8 @@ extern "C" int rb200_qkv_norm_post(const float* qkv, int qkv_stride, const float
     if (T == 0) return 0;
     RB_REQUIRE(qkv && q_out && k_pool && v_pool && m && m->pos && m->seq && m->table_off && m->tables && (rot_dim == 0 || inv_freq),
                "qkv_norm_post: null argument");
-    RB_REQUIRE(static_cast<const void*>(qkv) != q_out || qkv_stride == q_stride, "qkv_norm_post: q in place needs the same stride");
+    // a single row has no stride: torch, for one, reports a row's own width for a one-row view of wider rows
+    RB_REQUIRE(static_cast<const void*>(qkv) != q_out || qkv_stride == q_stride || T == 1, "qkv_norm_post: q in place needs the same stride");
     launch_qkv_norm_post(qkv, qkv_stride, bias, q_norm, k_norm, eps, inv_freq, rot_dim,
                          TokenMeta{m->pos, m->seq, m->table_off, m->tables}, T, q_out, q_stride, static_cast<__half*>(k_pool),
                          static_cast<__half*>(v_pool), heads, kv_heads, head_dim, block_size, as_stream(stream));
