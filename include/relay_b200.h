@@ -502,7 +502,8 @@ int rb200_argmax_rows(const float* logits, int R, int V, int32_t* token_out, flo
  * row, in this order (each part optional: NULL, or a leading dimension of 0, leaves it out):
  *  1. penalties: with the row's first history_len tokens of `history` ([R][ld_history]; the first
  *     prompt_len[r] of them are the prompt, all of them if it is larger, the others were generated),
- *     a token that occurs in it: x > 0 ? x / repetition : x * repetition; one generated count > 0
+ *     a token that occurs in it: x > 0 ? x / repetition : x * repetition (to the nearest float32 for
+ *     quotients between 2^-99 and 2^100, rounded twice outside); one generated count > 0
  *     times: x - (frequency * count + presence). `penalties` is a device array of R entries;
  *     prompt_len NULL: no prompt.
  *  2. bias_values[r][i] is added to token bias_ids[r][i], i < bias_len[r] ([R][ld_bias]); of

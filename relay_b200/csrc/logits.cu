@@ -30,11 +30,29 @@ struct LogitArgs {
   int ld_logits, ld_out, V, ld_history, ld_bias, ld_mask;
 };
 
-// `inverse`: 1 / repetition. The product with it may differ from the quotient in the last place.
-__device__ __forceinline__ float adjusted(float x, uint32_t c, const rb200_penalties& pen, float inverse) {
+// x / repetition for x > 0 without a division (56 us instead of 53.9 for 256 rows of 128256 logits; the product with the
+// reciprocal alone, 52, would be rounded twice). With repetition * scale in [1/2, 1) for a power of two `scale` (in
+// [2^-22, 1) where the repetition is subnormal) the quotient is z / (repetition * scale), z = x * scale. Its product with
+// the reciprocal is within 1.5 steps, and one residual step (Markstein's: r = z - q b in one rounding, q + r / b) brings
+// it to the nearest float32 but for 2^-22 of a step. Where r could underflow or q overflow the product stands.
+struct Repetition {
+  float value, scale, scaled, inverse;
+  __device__ __forceinline__ explicit Repetition(float repetition) : value(repetition) {
+    const int biased = 253 - static_cast<int>(__float_as_uint(repetition) >> 23 & 255u);  // exponent of the scale
+    scale = biased > 0 ? __uint_as_float(static_cast<uint32_t>(biased) << 23) : biased == 0 ? 0x1p-127f : 0x1p-128f;
+    scaled = repetition * scale;
+    inverse = 1.0f / scaled;
+  }
+  __device__ __forceinline__ float divides(float x) const {
+    const float z = x * scale, q = z * inverse, y = __fmaf_rn(__fmaf_rn(-q, scaled, z), inverse, q);
+    return z > 0x1p-100f && z < 0x1p100f ? y : q;
+  }
+};
+
+__device__ __forceinline__ float adjusted(float x, uint32_t c, const rb200_penalties& pen, const Repetition& rep) {
   const float times = static_cast<float>(c & ~kSeen);
   const float less = times > 0.0f ? pen.frequency * times + pen.presence : 0.0f;
-  return c ? x * (x > 0.0f ? inverse : pen.repetition) - less : x;
+  return c ? (x > 0.0f ? rep.divides(x) : x * rep.value) - less : x;
 }
 
 __device__ __forceinline__ bool allowed(const uint32_t* mask, int v) { return mask == nullptr || ((mask[v >> 5] >> (v & 31)) & 1u); }
@@ -123,7 +141,7 @@ adjust_logits_kernel(const LogitArgs a) {
 
   // The values, B vectors of a thread at a time: 51 us for 256 rows of 128256 logits. (All of them on their way ahead of
   // the count leave registers for two CTAs to an SM instead of three: 63. The first B ahead of it spill: 69.)
-  const float inverse = 1.0f / pen.repetition;
+  const Repetition rep(pen.repetition);
   constexpr int B = NV < 4 ? NV : 4;
 #pragma unroll
   for (int n0 = 0; n0 < NV; n0 += B) {
@@ -151,8 +169,8 @@ adjust_logits_kernel(const LogitArgs a) {
         const uint4 c = *reinterpret_cast<const uint4*>(count + at);
         if (c.x | c.y | c.z | c.w) {
           changed = true;
-          val[j].x = adjusted(val[j].x, c.x, pen, inverse), val[j].y = adjusted(val[j].y, c.y, pen, inverse);
-          val[j].z = adjusted(val[j].z, c.z, pen, inverse), val[j].w = adjusted(val[j].w, c.w, pen, inverse);
+          val[j].x = adjusted(val[j].x, c.x, pen, rep), val[j].y = adjusted(val[j].y, c.y, pen, rep);
+          val[j].z = adjusted(val[j].z, c.z, pen, rep), val[j].w = adjusted(val[j].w, c.w, pen, rep);
         }
       }
       if (!changed) continue;

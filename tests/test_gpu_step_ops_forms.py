@@ -5,7 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from tests.test_gpu_step_ops import NORM_TOL, dev, norm_rope_f64, ops  # noqa: E402, F401
+from tests.test_gpu_step_ops import NORM_TOL, U32, dev, norm_rope_f64, ops  # noqa: E402, F401
 
 
 @pytest.mark.parametrize("T", [1, 2, 5])
@@ -27,3 +27,47 @@ def test_qkv_norm_post_in_place_through_a_view_of_the_query_part(ops, T):  # noq
     assert np.all(np.abs(after[:, :heads * D].reshape(q.shape) - q) <= NORM_TOL * reach[:, :heads])
     assert np.array_equal(after[:, heads * D:], x[:, heads * D:])
     assert np.array_equal(pools[1].cpu().numpy()[0, :, 9:9 + T].transpose(1, 0, 2), v.astype(np.float16))
+
+
+def check_penalised(got, x, rep):
+    """`got` against x / rep for x > 0 and x rep for the others, in float64."""
+    wide, rep = x.astype(np.float64), rep.astype(np.float64)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = np.where(wide > 0, wide / rep, wide * rep)
+        nearest = want.astype(np.float32)
+    finite = np.isfinite(nearest)
+    assert np.array_equal(got[~finite], nearest[~finite], equal_nan=True)
+    # Half a step of float32 (2^-22 of one more for a quotient), or of its subnormals. Quotients outside of 2^-99 to 2^100
+    # are products with a reciprocal: each of the two rounds, and where the type's range ends below so does the
+    # scaled logit (half a subnormal step, times a reciprocal of at most 2).
+    size = np.abs(want[finite])
+    twice = (wide[finite] > 0) & ((size <= 2.0 ** -99) | (size >= 2.0 ** 100))
+    tol = np.where(twice, 2 * U32 * size + 3 * 2.0 ** -150, U32 * (1 + 2.0 ** -22) * size + 2.0 ** -150)
+    assert np.all(np.abs(got[finite] - want[finite]) <= tol)
+
+
+@pytest.mark.parametrize("repetition", [1e-39, 2.0 ** -128, 0.7, 1.1, 3.0, 1e38])
+def test_adjust_logits_divides_by_the_repetition(ops, repetition):  # noqa: F811
+    # also where 1 / repetition is no float32
+    R, V = 3, 5000
+    x = np.random.Generator(np.random.PCG64(2)).standard_normal((R, V)).astype(np.float32)
+    x *= np.float32(1e-3 if repetition < 1 else 4)
+    pen = np.zeros((R, 4), np.float32)
+    pen[:, 0] = repetition
+    history = np.broadcast_to(np.arange(V, dtype=np.int32), (R, V))
+    out = torch.empty((R, V), device="cuda")
+    ops.adjust_logits(dev(x), out, dev(pen), dev(history), dev(np.full(R, V, np.int32)))
+    check_penalised(out.cpu().numpy(), x, pen[:, :1])
+
+
+def test_adjust_logits_divides_by_the_repetition_at_every_magnitude(ops):  # noqa: F811
+    rng = np.random.Generator(np.random.PCG64(7))
+    R, V = 120, 3001
+    x = (rng.standard_normal((R, V)) * 2.0 ** rng.integers(-140, 120, (R, V))).astype(np.float32)
+    x[:, 0], x[:, 1], x[:, 2] = np.inf, -np.inf, np.nan
+    pen = np.zeros((R, 4), np.float32)
+    pen[:, 0] = (1 + rng.random(R)) * 2.0 ** rng.integers(-30, 30, R)
+    history = np.broadcast_to(np.arange(V, dtype=np.int32), (R, V))
+    out = torch.empty((R, V), device="cuda")
+    ops.adjust_logits(dev(x), out, dev(pen), dev(history), dev(np.full(R, V, np.int32)))
+    check_penalised(out.cpu().numpy(), x, pen[:, :1])
