@@ -125,7 +125,7 @@ qkv_norm_pair_kernel(const float* qkv, const float* __restrict__ bias, const flo
             *reinterpret_cast<float4*>(dst + h * D) = make_float4(y0.a.x, y0.a.y, y0.b.x, y0.b.y);
             *reinterpret_cast<float4*>(dst + h * D + D / 2) = make_float4(y1.a.x, y1.a.y, y1.b.x, y1.b.y);
           } else {
-            __half* to = (is_v ? vc : kc) + page + (is_v ? h - heads - kv_heads : h - heads) * bs * D;
+            __half* to = (is_v ? vc : kc) + page + static_cast<long long>(is_v ? h - heads - kv_heads : h - heads) * bs * D;
             *reinterpret_cast<uint2*>(to) = make_uint2(pack_half2(y0.a.x, y0.a.y), pack_half2(y0.b.x, y0.b.y));
             *reinterpret_cast<uint2*>(to + D / 2) = make_uint2(pack_half2(y1.a.x, y1.a.y), pack_half2(y1.b.x, y1.b.y));
           }
@@ -262,7 +262,7 @@ qkv_norm_vec_kernel(const float* qkv, const float* __restrict__ bias, const floa
           *reinterpret_cast<float4*>(dst + h * D + n * LPH * 4) = x[u][n];
         } else {
           const int kvh = is_v ? h - heads - kv_heads : h - heads;
-          *reinterpret_cast<uint2*>((is_v ? vc : kc) + page + kvh * bs * D + (l + n * LPH) * 4) =
+          *reinterpret_cast<uint2*>((is_v ? vc : kc) + page + static_cast<long long>(kvh) * bs * D + (l + n * LPH) * 4) =
               make_uint2(pack_half2(x[u][n].x, x[u][n].y), pack_half2(x[u][n].z, x[u][n].w));
         }
       }

@@ -5,7 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from tests.test_gpu_step_ops import NORM_TOL, U32, dev, norm_rope_f64, ops  # noqa: E402, F401
+from tests.test_gpu_step_ops import H16, NORM_TOL, U32, dev, norm_rope_f64, ops  # noqa: E402, F401
 
 
 @pytest.mark.parametrize("T", [1, 2, 5])
@@ -71,3 +71,25 @@ def test_adjust_logits_divides_by_the_repetition_at_every_magnitude(ops):  # noq
     out = torch.empty((R, V), device="cuda")
     ops.adjust_logits(dev(x), out, dev(pen), dev(history), dev(np.full(R, V, np.int32)))
     check_penalised(out.cpu().numpy(), x, pen[:, :1])
+
+
+@pytest.mark.parametrize("D,bs", [(128, 1 << 23), (80, 1 << 24), (66, 1 << 24)])
+def test_qkv_norm_post_into_a_block_of_more_than_2_31_values(ops, D, bs):  # noqa: F811
+    # one block per sequence, as long as its context may get: the third KV head begins 2^31 values in or later
+    heads, kv_heads, T = 2, 3, 3
+    rng = np.random.Generator(np.random.PCG64(D))
+    x = rng.standard_normal((T, (heads + 2 * kv_heads) * D)).astype(np.float32)
+    pos = np.asarray([0, bs - 2, bs - 1])
+    inv = (500000.0 ** -(np.arange(0, D, 2) / D)).astype(np.float32)
+    pools = [torch.zeros((1, kv_heads, bs, D), dtype=torch.float16, device="cuda") for _ in range(2)]
+    q_out = torch.empty((T, heads * D), device="cuda")
+    ops.qkv_norm_post(dev(x), None, None, None, 1e-6, dev(inv), ops.TokenMeta.from_host(pos, np.zeros(T), [0], [0]), q_out, *pools,
+                      heads, kv_heads, D, bs)
+    q, k, v, reach = norm_rope_f64(x, None, None, None, 1e-6, inv, pos, heads, kv_heads, D, D)
+    assert np.all(np.abs(q_out.cpu().numpy().reshape(q.shape) - q) <= NORM_TOL * reach[:, :heads])
+    got = [pool[0][:, torch.from_numpy(pos).cuda()].cpu().numpy().transpose(1, 0, 2) for pool in pools]
+    tol = H16 * np.abs(k) + 2.0 ** -25 + NORM_TOL * reach[:, heads:heads + kv_heads]
+    assert np.all(np.abs(got[0].astype(np.float64) - k) <= tol)
+    assert np.array_equal(got[1], v.astype(np.float16))
+    for pool, here in zip(pools, got):  # nothing went anywhere else
+        assert sum(int(torch.count_nonzero(pool[0, h])) for h in range(kv_heads)) == np.count_nonzero(here)
