@@ -106,7 +106,14 @@ struct PerDeviceOnce {
 // the first kernel of a pass, or is updated by session_advance_kernel / session_finish_kernel, and
 // session_advance_kernel does not call pdl_trigger(): the kernel behind it, and with it every
 // later kernel of the step, starts only once the update is complete. Activations and K/V pages
-// are written by kernels of the same pass and are read after the wait only.
+// are written by kernels of the same pass and are read after the wait only, with one exception:
+// a kernel whose predecessor calls pdl_trigger() only BEHIND its own pdl_wait(), in every CTA,
+// starts when all that ran ahead of the predecessor is complete and in L2, so it may read that
+// (not what the predecessor itself writes) ahead of its own wait, by loads that go to L2 (__ldcg,
+// cp.async.cg): nothing has been said about this SM's L1 yet. That holds for the kernel behind it,
+// too, if it triggers ahead of its wait. Such a kernel still waits in at least one CTA, so that it
+// does not complete ahead of its predecessor. The suffix kernel of shared_prefix.cu (metadata, q,
+// pages) and its join kernel (metadata) rely on it.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

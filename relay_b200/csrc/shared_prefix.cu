@@ -264,14 +264,14 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
 
   __half* ring = reinterpret_cast<__half*>(smem_raw) + static_cast<size_t>(warp) * S * 2 * TILE_HALVES;
   const uint32_t ring_u32 = smem_u32(ring);
-  // Tiles warp, warp + W, ... of the slice belong to this warp. Where a tile lies in one page, its
-  // block id waits in a register: 32 tiles' ids at a time, one per lane, the next 32 on their way.
+  // Tiles warp, warp + W, ... of the slice belong to this warp. Block ids wait in registers, read ahead of their use
+  // and from L2: where a tile lies in one page 32 tiles' ids, one per lane, otherwise those of a tile's 16 keys.
   const int my_tiles = ntiles > warp ? (ntiles - warp + W - 1) / W : 0;
   auto fetch_ids = [&](int j0) {
-    const int j = j0 + lane, key = k0 + (warp + j * W) * 16;
-    return CONTIG && j < my_tiles ? __ldcg(table + (bs_shift >= 0 ? key >> bs_shift : key / bs)) : 0;
+    const int j = CONTIG ? j0 + lane : j0, key = k0 + (warp + j * W) * 16 + (CONTIG ? 0 : lane & 15);
+    return j < my_tiles && key < k1 ? __ldcg(table + (bs_shift >= 0 ? key >> bs_shift : key / bs)) : 0;
   };
-  int ids = fetch_ids(0), ids_next = fetch_ids(32);
+  int ids = fetch_ids(0), ids_next = fetch_ids(CONTIG ? 32 : 1);
   auto load_tile = [&](int j) {
     const uint32_t kdst = ring_u32 + static_cast<uint32_t>(j % S) * 2 * TILE_HALVES * 2;
     const uint32_t vdst = kdst + TILE_HALVES * 2;
@@ -294,15 +294,19 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
         cp_async16_zfill(vdst + off, vc + at + (bytes ? idx * 8 : 0), bytes);
       }
     } else {
+      const int mine = ids;  // of this tile: tiles are loaded in order
+      ids = ids_next;
+      ids_next = fetch_ids(j + 2);
 #pragma unroll
       for (int idx = lane; idx < 16 * CH; idx += 32) {
         const int row = idx / CH, c = idx % CH;
-        const bool ok = row < nvalid;
-        const long long at = ok ? key_offset(table, 0, key0 + row, bs, bs_shift, kv_heads, kvh, D) : 0;
-        const int bytes = ok ? 16 : 0;
+        const long long block = __shfl_sync(0xffffffffu, mine, row);
+        const int key = key0 + row, slot = bs_shift >= 0 ? key & (bs - 1) : key % bs;
+        const int bytes = row < nvalid ? 16 : 0;
+        const long long at = bytes ? ((block * kv_heads + kvh) * bs + slot) * D + c * 8 : 0;
         const uint32_t off = static_cast<uint32_t>(swz<CH>(row, c)) * 16;
-        cp_async16_zfill(kdst + off, kc + at + c * 8, bytes);
-        cp_async16_zfill(vdst + off, vc + at + c * 8, bytes);
+        cp_async16_zfill(kdst + off, kc + at, bytes);
+        cp_async16_zfill(vdst + off, vc + at, bytes);
       }
     }
   };

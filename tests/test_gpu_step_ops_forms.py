@@ -5,7 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from tests.test_gpu_step_ops import H16, NORM_TOL, U32, dev, norm_rope_f64, ops  # noqa: E402, F401
+from tests.test_gpu_step_ops import (H16, NORM_TOL, SHARED, U32, check_prefix, dev, norm_rope_f64, ops,  # noqa: E402, F401
+                                     prefix_case)
 
 
 @pytest.mark.parametrize("T", [1, 2, 5])
@@ -93,3 +94,38 @@ def test_qkv_norm_post_into_a_block_of_more_than_2_31_values(ops, D, bs):  # noq
     assert np.array_equal(got[1], v.astype(np.float16))
     for pool, here in zip(pools, got):  # nothing went anywhere else
         assert sum(int(torch.count_nonzero(pool[0, h])) for h in range(kv_heads)) == np.count_nonzero(here)
+
+
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 24), (64, 8), (32, 8), (16, 1)])
+def test_shared_prefix_attention_follows_tables_rewritten_in_place(ops, D, bs):  # noqa: F811
+    # a captured step whose block tables, pages and queries change between replays, in kernels and copies just ahead of it
+    c = prefix_case(31, D, 8, 2, bs, [(900, [1, 40, 333]), (70, [5, 200])])
+    shape = ops.attn_shape(8, 2, D, bs, o_stride=c["o_stride"])
+    meta = ops.TokenMeta.from_host(c["pos"], c["seq"], c["table_off"], c["tables"])
+    pools = [dev(np.nan_to_num(c[name])) for name in ("k", "v")]
+    tables, pages, queries = meta.tables.clone(), [p.clone() for p in pools], dev(c["q"])
+    q, out = queries.clone(), torch.full((len(c["pos"]), c["o_stride"]), 7.0, dtype=torch.float16, device="cuda")
+    scratch = torch.empty(ops.shared_prefix_scratch_bytes(shape, 5, 2, *SHARED), dtype=torch.uint8, device="cuda")
+    args = dev(c["tokens"]), dev(c["off"]), dev(c["lens"]), *SHARED, *pools, out, scratch
+    nb = len(c["k"])
+    order = torch.arange(nb, device="cuda")
+
+    def step():
+        # the same batch with its blocks elsewhere in the pool
+        meta.tables.copy_(order[tables.long()].int())
+        for pool, page in zip(pools, pages):
+            pool[order] = page
+        q.copy_(queries)
+        ops.shared_prefix_attention(shape, q, meta, *args)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for shift in range(8):
+        order.copy_((torch.arange(nb, device="cuda") + 3 * shift) % nb)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_prefix(c, out.cpu().numpy(), 7.0)
