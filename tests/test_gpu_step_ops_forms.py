@@ -6,7 +6,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from tests.test_gpu_step_ops import (H16, NORM_TOL, SHARED, U32, check_prefix, dev, norm_rope_f64, ops,  # noqa: E402, F401
-                                     prefix_case)
+                                     padded, prefix_case, run_prefix)
 
 
 @pytest.mark.parametrize("T", [1, 2, 5])
@@ -129,3 +129,83 @@ def test_shared_prefix_attention_follows_tables_rewritten_in_place(ops, D, bs): 
         graph.replay()
         torch.cuda.synchronize()
         check_prefix(c, out.cpu().numpy(), 7.0)
+
+
+# ---- queries that fp16 does not hold -------------------------------------------------------------
+
+HOT = 60.0  # score of two keys of each context; all others score 0
+
+
+def competing_case(seed, D, heads, kv_heads, bs, groups, where):
+    """A prefix_case in which two keys of each context share the weight, their scores nearly equal and so large that
+    rounding the query to fp16 would move the weights visibly. `where`: 's' and 'o' for shared and own keys."""
+    c = prefix_case(seed, D, heads, kv_heads, bs, groups, dtype_q=np.float32)
+    rng = np.random.Generator(np.random.PCG64(seed))
+    n = len(c["q"])
+    c["q"][:, :heads * D] = 30 * (1 + 2.0 ** -9 * rng.uniform(-1, 1, (n, heads * D)))  # some seven steps of fp16 wide
+    c["k"][~np.isnan(c["k"])] = 0
+    hot = np.float16(HOT * np.sqrt(D) / 30)
+    i = 0
+    for P, own in groups:
+        shared = rng.permutation(P)[:2]
+        for s in own:
+            ctx, tok = c["contexts"][i], c["tokens"][i]
+            ctx[0] = 0
+            mine = P + rng.permutation(s)[:2]
+            for j, (kind, dim) in enumerate(zip(where, (3, D - 2))):  # each of the two keys looks at one dimension
+                key = shared[j] if kind == "s" else mine[j]
+                page = c["tables"][c["table_off"][c["seq"][tok]] + key // bs]
+                ctx[0, key, :, dim] = c["k"][page, :, key % bs, dim] = hot
+            i += 1
+    return c
+
+
+def check_unrounded(c, out):
+    """Each decode token against float64, with nothing granted for a rounding of q; and what such a rounding would do."""
+    D, G = c["D"], c["heads"] // c["kv_heads"]
+
+    def attend(q, ctx):
+        k, v = (ctx[i].astype(np.float64).transpose(1, 0, 2) for i in (0, 1))
+        s = q.reshape(c["kv_heads"], G, D) @ k.transpose(0, 2, 1) / np.sqrt(D)
+        w = np.exp(s - s.max(-1, keepdims=True))
+        total = w.sum(-1, keepdims=True)
+        return w / total @ v, w / total @ np.abs(v), total
+
+    for tok, ctx in zip(c["tokens"], c["contexts"]):
+        q = c["q"][tok, :c["heads"] * D]
+        want, spread, total = attend(q.astype(np.float64), ctx)
+        # Weights and output round to fp16 (2^-11 each; weights below 2^-14 of the largest to 2^-25). Scores are single
+        # products: q = hi + lo to 2^-22, three roundings to float32, 60 (2^-22 + 3 2^-24) = 2.5e-5 < 2^-15; such an
+        # error of both scores moves the output by 2^-15 of the spread at most, as do exponentials and sums.
+        tol = (H16 + 2 * 2.0 ** -15) * spread + H16 * np.abs(want) + ctx.shape[1] * 2.0 ** -25 * np.abs(ctx[1]).max() / total + 2.0 ** -25
+        rounded, _, _ = attend(q.astype(np.float16).astype(np.float64), ctx)
+        assert (np.abs(rounded - want) / tol).max() > 4, "the case would not notice a query rounded to fp16"
+        if out is not None:
+            got = out[tok, :c["heads"] * D].astype(np.float64).reshape(want.shape)
+            assert (np.abs(got - want) / tol).max() <= 1, (tok, (np.abs(got - want) / tol).max())
+
+
+COMPETING = [
+    # D, heads, kv_heads, bs, groups
+    (128, 32, 8, 16, [(700, [5, 40]), (130, [2, 17, 300])]),
+    (128, 32, 8, 16, [(700, [2 + i for i in range(40)])]),   # more than 64 rows to a group
+    (64, 10, 2, 16, [(700, [5, 40]), (130, [2, 17, 300])]),
+    (64, 10, 2, 16, [(700, [2 + i for i in range(40)])]),
+    (128, 8, 2, 8, [(500, [5, 40, 130])]),
+    (64, 32, 2, 24, [(500, [5, 40, 130])]),
+    (32, 8, 2, 8, [(500, [5, 40, 130])]),
+    (32, 32, 2, 16, [(500, [5, 40, 130])]),
+    (16, 16, 1, 8, [(500, [5, 40, 130])]),
+]
+
+
+@pytest.mark.parametrize("where", ["ss", "oo", "so"])
+@pytest.mark.parametrize("D,heads,kv_heads,bs,groups", COMPETING)
+def test_shared_prefix_attention_takes_queries_in_full(ops, D, heads, kv_heads, bs, groups, where):  # noqa: F811
+    c = competing_case(D + heads, D, heads, kv_heads, bs, groups, where)
+    check_unrounded(c, run_prefix(ops, c))
+    check_unrounded(c, run_prefix(ops, c, SHARED))
+    check_unrounded(c, run_prefix(ops, c, (0, c["max_prefix"] + c["max_suffix"])))
+    wide = padded(c)
+    check_unrounded(c, run_prefix(ops, wide))
+    check_unrounded(c, run_prefix(ops, wide, (0, c["max_prefix"] + c["max_suffix"])))
