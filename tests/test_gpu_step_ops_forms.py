@@ -5,6 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+from tests import test_gpu_step_ops as base  # noqa: E402
 from tests.test_gpu_step_ops import (H16, NORM_TOL, SHARED, U32, check_prefix, dev, norm_rope_f64, ops,  # noqa: E402, F401
                                      padded, prefix_case, run_prefix)
 
@@ -209,3 +210,119 @@ def test_shared_prefix_attention_takes_queries_in_full(ops, D, heads, kv_heads, 
     wide = padded(c)
     check_unrounded(c, run_prefix(ops, wide))
     check_unrounded(c, run_prefix(ops, wide, (0, c["max_prefix"] + c["max_suffix"])))
+
+
+# ---- every form of the kernels -------------------------------------------------------------------
+
+FEW, MANY = [(40, 3), (7, 1), (0, 2)], [(29, 500), (3, 211), (1000, 1)]
+
+QKV_FORMS = [
+    # D, heads, kv_heads, bs, rot, bias, norms
+    # two vectors of a head to a lane: rotated whole, by half
+    (32, 7, 3, 8, 32, True, "qk"), (32, 7, 3, 8, 16, False, "qk"),
+    (64, 9, 2, 16, 64, True, "qk"), (64, 9, 2, 16, 32, True, "k"),
+    (128, 12, 4, 16, 128, True, "qk"), (128, 12, 4, 16, 64, True, "qk"), (128, 5, 5, 48, 64, False, "q"),
+    (256, 3, 1, 16, 256, True, "qk"), (256, 3, 1, 16, 128, True, "qk"),
+    # vectors by shuffle: 8, 16 and 32 lanes to a head, two vectors to a lane
+    (24, 7, 3, 8, 24, True, "qk"), (32, 7, 3, 8, 8, True, "qk"),
+    (48, 7, 3, 8, 48, True, "qk"), (64, 9, 2, 16, 16, True, "qk"), (36, 5, 2, 16, 24, False, "k"),
+    (96, 7, 3, 16, 96, True, "qk"), (128, 7, 3, 16, 32, True, "q"),
+    (192, 3, 2, 16, 96, True, "qk"), (160, 3, 2, 16, 160, True, "qk"), (256, 3, 1, 16, 64, True, "qk"),
+    # value by value
+    (34, 7, 3, 8, 34, True, "qk"), (66, 7, 3, 16, 20, True, "qk"), (250, 3, 1, 16, 250, True, "q"), (128, 3, 1, 16, 12, True, "qk"),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("chunks", [FEW, MANY])
+@pytest.mark.parametrize("D,heads,kv_heads,bs,rot,use_bias,norms", QKV_FORMS)
+def test_qkv_norm_post_in_every_form(ops, D, heads, kv_heads, bs, rot, use_bias, norms, chunks, in_place):  # noqa: F811
+    base.test_qkv_norm_post(ops, D, heads, kv_heads, bs, rot, use_bias, norms, chunks, in_place)
+
+
+@pytest.mark.parametrize("D,heads,kv_heads,bs,rot,use_bias,norms", QKV_FORMS[:9])
+def test_qkv_norm_post_of_more_tokens_than_a_grid_in_every_form(ops, D, heads, kv_heads, bs, rot, use_bias, norms):  # noqa: F811
+    # up to 32 CTAs are on an SM: some of them go through two tokens, or with more heads through several
+    base.test_qkv_norm_post(ops, D, heads, kv_heads, bs, rot, use_bias, norms, [(29, 5200)], True)
+
+
+PREFIX_FORMS = [
+    # D, heads, kv_heads, bs, groups: blocks that 16 divides and does not divide, up to 8 heads to a KV head and up to 16
+    (D, heads, kv_heads, bs, groups)
+    for D in (128, 64, 32, 16)
+    for heads, kv_heads in ((10, 2), (24, 2))
+    for bs in (16, 24, 8)
+    for groups in ([(777, [1, 30, 200, None]), (50, []), (129, [2] * 7), (0, [40]), (9, [])],)
+]
+
+
+@pytest.mark.parametrize("D,heads,kv_heads,bs,groups", PREFIX_FORMS)
+def test_shared_prefix_attention_in_every_form(ops, D, heads, kv_heads, bs, groups):  # noqa: F811
+    c = prefix_case(D + bs, D, heads, kv_heads, bs, groups)
+    wide, alone = padded(c), (0, c["max_prefix"] + c["max_suffix"])
+    for batch, hints in ((c, None), (c, SHARED), (c, alone), (wide, None), (wide, alone)):
+        check_prefix(c, run_prefix(ops, batch, hints), 7.0)
+
+
+@pytest.mark.parametrize("hints", [None, SHARED, (0, 1000)])
+@pytest.mark.parametrize("groups", [[(40, []), (300, [5, 70])], [(300, [5]), (8, []), (8, []), (17, [1, 2])],
+                                    [(0, [])] * 40 + [(200, [3, 9])] + [(5, [])] * 40])
+def test_shared_prefix_attention_with_groups_of_nobody(ops, groups, hints):  # noqa: F811
+    c = prefix_case(33, 64, 8, 2, 16, groups)
+    check_prefix(c, run_prefix(ops, c, hints), 7.0)
+
+
+def test_refusals_of_device_tensors_launch_nothing(ops):  # noqa: F811
+    from relay_b200 import _lib
+    f32, f16, i32 = (dict(dtype=t, device="cuda") for t in (torch.float32, torch.float16, torch.int32))
+    T, H, KV, D, bs, V = 3, 4, 2, 64, 16, 100
+    width = (H + 2 * KV) * D
+    meta = ops.TokenMeta(*(torch.zeros(n, **i32) for n in (T, T, 1, 1)))
+    short = ops.TokenMeta(meta.pos[:2], meta.seq, meta.table_off, meta.tables)
+    host = ops.TokenMeta(meta.pos.cpu(), meta.seq, meta.table_off, meta.tables)
+    pool = torch.zeros(2, KV, bs, D, **f16)
+    qkv, q, out, inv, norm = torch.zeros(T, width, **f32), torch.zeros(T, H * D, **f32), torch.zeros(T, H * D, **f16), torch.zeros(32, **f32), torch.ones(D, **f32)
+
+    def norm_post(**kw):
+        a = dict(qkv=qkv, bias=None, q_norm=norm, k_norm=norm, eps=1e-6, inv_freq=inv, meta=meta, q_out=q, k_pool=pool, v_pool=pool,
+                 heads=H, kv_heads=KV, head_dim=D, block_size=bs, rot_dim=None)
+        ops.qkv_norm_post(**(a | kw))
+
+    def prefix(**kw):
+        a = dict(shape=ops.attn_shape(H, KV, D, bs, q_stride=H * D), q=q, meta=meta, decode_tokens=torch.arange(T, **i32),
+                 group_off=torch.tensor([0, T], **i32), prefix_len=torch.zeros(1, **i32), max_prefix=0, max_suffix=1, k_pool=pool, v_pool=pool,
+                 out=out, scratch=None)
+        ops.shared_prefix_attention(**(a | kw))
+
+    logits = torch.zeros(T, V, **f32)
+    ids, lens = torch.zeros(T, 5, **i32), torch.zeros(T, **i32)
+
+    def adjust(**kw):
+        a = dict(logits=logits, out=logits, penalties=torch.ones(T, 4, **f32), history=ids, history_len=lens, prompt_len=lens, bias_ids=ids,
+                 bias_values=torch.zeros(T, 5, **f32), bias_len=lens, mask=torch.zeros(T, 4, **i32))
+        ops.adjust_logits(**(a | kw))
+
+    refused = [
+        (norm_post, dict(qkv=qkv.half()), "float32"), (norm_post, dict(qkv=qkv[:, 1:]), "head_dim"), (norm_post, dict(qkv=qkv.t().contiguous().t()), "contiguous"),
+        (norm_post, dict(q_out=q[:2]), "q_out"), (norm_post, dict(meta=short), "metadata"), (norm_post, dict(meta=host), "device"),
+        (norm_post, dict(k_pool=pool[:, :1].contiguous()), "pools"), (norm_post, dict(v_pool=pool[:1]), "pools"), (norm_post, dict(v_pool=pool.transpose(1, 2)), "contiguous"),
+        (norm_post, dict(bias=norm), "bias"), (norm_post, dict(k_norm=inv), "q_norm and k_norm"), (norm_post, dict(rot_dim=32), "inv_freq"),
+        (norm_post, dict(rot_dim=66, inv_freq=torch.zeros(33, **f32)), "rot_dim"),
+        (prefix, dict(q=q[:2]), "rows"), (prefix, dict(out=out[:2]), "rows"), (prefix, dict(out=out.float()), "float16"), (prefix, dict(q=qkv), "apart"),
+        (prefix, dict(group_off=torch.zeros(3, **i32)), "group_off"), (prefix, dict(decode_tokens=torch.arange(T, device="cuda")), "int32"),
+        (prefix, dict(k_pool=pool[:, :, :8].contiguous()), "pools"), (prefix, dict(scratch=torch.zeros(8, **f32)), "uint8"), (prefix, dict(max_prefix=-1), "bad batch"),
+        (prefix, dict(max_prefix=100000, scratch=torch.zeros(16, dtype=torch.uint8, device="cuda")), "scratch too small"),
+        (adjust, dict(out=torch.zeros(T, V + 1, **f32)), "vocabulary"), (adjust, dict(out=torch.zeros(1, V, **f32).expand(T, V)), "shorter"),
+        (adjust, dict(penalties=torch.ones(T, 3, **f32)), "penalties"), (adjust, dict(history=None), "history"), (adjust, dict(history_len=lens[:2]), "history"),
+        (adjust, dict(history=ids.long()), "int32"), (adjust, dict(bias_values=None), "bias_ids"), (adjust, dict(bias_len=lens[:1]), "bias_ids"),
+        (adjust, dict(mask=torch.zeros(T, 3, **i32)), "mask"), (adjust, dict(mask=torch.zeros(1, 4, **i32)), "mask"),
+    ]
+    before = _lib.lib().rb200_kernel_launches()
+    for call, kw, text in refused:
+        with pytest.raises(ValueError, match=text):
+            call(**kw)
+    assert _lib.lib().rb200_kernel_launches() == before
+    for call in (norm_post, prefix, adjust):
+        call()
+    torch.cuda.synchronize()
+    assert _lib.lib().rb200_kernel_launches() == before + 3
