@@ -297,11 +297,12 @@ suffix_kernel(const float* __restrict__ q, TokenMeta m, Groups gr, const __half*
       const int mine = ids;  // of this tile: tiles are loaded in order
       ids = ids_next;
       ids_next = fetch_ids(j + 2);
+      const int my_slot = bs_shift >= 0 ? 0 : (key0 + (lane & 15)) % bs;
 #pragma unroll
       for (int idx = lane; idx < 16 * CH; idx += 32) {
         const int row = idx / CH, c = idx % CH;
         const long long block = __shfl_sync(0xffffffffu, mine, row);
-        const int key = key0 + row, slot = bs_shift >= 0 ? key & (bs - 1) : key % bs;
+        const int slot = bs_shift >= 0 ? (key0 + row) & (bs - 1) : __shfl_sync(0xffffffffu, my_slot, row);
         const int bytes = row < nvalid ? 16 : 0;
         const long long at = bytes ? ((block * kv_heads + kvh) * bs + slot) * D + c * 8 : 0;
         const uint32_t off = static_cast<uint32_t>(swz<CH>(row, c)) * 16;
