@@ -139,8 +139,9 @@ adjust_logits_kernel(const LogitArgs a) {
     __syncthreads();
   }
 
-  // The values, B vectors of a thread at a time: 51 us for 256 rows of 128256 logits. (All of them on their way ahead of
-  // the count leave registers for two CTAs to an SM instead of three: 63. The first B ahead of it spill: 69.)
+  // The values, B vectors of a thread at a time. (All of them on their way ahead of the count leave registers for two CTAs
+  // to an SM instead of three: 63 us for 256 rows of 128256 logits against 51, measured with a reciprocal in place of the
+  // quotient. The first B ahead of it spill: 69.)
   const Repetition rep(pen.repetition);
   constexpr int B = NV < 4 ? NV : 4;
 #pragma unroll
@@ -232,10 +233,10 @@ void launch_adjust_logits(const float* logits, int ld_logits, float* out, int ld
                     ld_logits, ld_out, V, ld_history, ld_bias, ld_mask};
   // Every segment reads its row's whole history, so segments are as long as leaves the GPU busy: three CTAs for every SM
   // in segments of 16384, two in 8192, one in 4096, otherwise 2048. Measured at 128256 logits and histories of 8192:
-  // 256 rows 57, 70, 99 and 153 us in 16384, 8192, 4096 and 2048; 32 rows 11.8 in 8192, 13.9 in 4096; 16 rows 8.7 and 8.8;
-  // 8 rows 6.8 in 4096, 7.5 in 2048; one row with 800 tokens 3.9 and 3.5.
+  // 256 rows 59, 72, 99 and 153 us in 16384, 8192, 4096 and 2048; 32 rows 13.5 in 8192, 15.0 in 4096; 16 rows 9.8 and 9.2;
+  // 8 rows 7.3 in 4096, 7.4 in 2048; one row with 800 tokens 4.3 and 3.8.
   // (Clusters that read a history once and count in the owner's shared memory: 119 us for 256 rows; a list of the counted
-  // tokens, whose values alone are adjusted once the others are stored: 77, against 51 with histories of 40 - 8192.)
+  // tokens, whose values alone are adjusted once the others are stored: 77, against 51 then, with histories of 40 - 8192.)
   const long long places = V + 3LL, sms = sm_count();
   if (R * (places / (kLgThreads * 32)) >= 3 * sms) launch_segments<8>(a, R, st);
   else if (R * (places / (kLgThreads * 16)) >= 2 * sms) launch_segments<4>(a, R, st);

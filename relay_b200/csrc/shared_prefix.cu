@@ -606,8 +606,9 @@ size_t scratch_of(const AttnShape& s, int n_decode, const Plan& p) {
 //    with 128 - 640 of their own, 105 us in one slice (64 CTAs beside the own keys) and 117 in two, which fill the
 //    GPU; 32 tokens behind 4096 with 64 - 512: 24, 20.5, 25 and 28 us in 4, 8, 11 and 16 slices;
 //  * the suffix kernel takes kOwnStartUs and for every key of a slice 5 ns and 35 ps a value of the head (blocks that
-//    16 keys do not divide: 2.5 ns more), 0.6 of that in CTAs of eight warps (`wide`); with x CTAs to an SM 0.65 + x / 2
-//    times as much (heads of 64 and less: 0.65 + 0.35 x). Slices take kOwnJoinUs more;
+//    16 keys do not divide: 2.5 ns more; measured with blocks of 8, 2 more at heads of 32, 4 at 64, 7 at 128), 0.6 of that
+//    in CTAs of eight warps (`wide`); with x CTAs to an SM 0.65 + x / 2 times as much (heads of 64 and less: 0.65 + 0.35 x).
+//    Slices take kOwnJoinUs more;
 //  * a launch behind the first counts kLaunchUs, most of the 2.5 us of the caller's time for it, which a graph does
 //    not spend.
 // Measured over 400 batches of 1 - 512 tokens in 1 - 64 groups behind 64 - 3000 keys in five head layouts, where the plan
