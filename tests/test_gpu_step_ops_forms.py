@@ -1,4 +1,8 @@
 """The decode-step operators around a shared prompt in the forms that test_gpu_step_ops.py does not reach."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -326,3 +330,41 @@ def test_refusals_of_device_tensors_launch_nothing(ops):  # noqa: F811
         call()
     torch.cuda.synchronize()
     assert _lib.lib().rb200_kernel_launches() == before + 3
+
+
+FIRST_CALLS_FROM_SEVERAL_THREADS = """
+import threading
+import torch
+from relay_b200 import ops
+i32 = dict(dtype=torch.int32, device="cuda")
+shape = ops.attn_shape(8, 2, 128, 16)
+pool = torch.randn(40, 2, 16, 128, device="cuda").half()
+q = torch.randn(1, 12 * 128, device="cuda")
+meta = ops.TokenMeta(torch.tensor([599], **i32), torch.tensor([0], **i32), torch.tensor([0], **i32), torch.arange(40, **i32))
+args = shape, q, meta, torch.tensor([0], **i32), torch.tensor([0, 1], **i32), torch.tensor([590], **i32)
+logits = torch.randn(300, 60000, device="cuda")
+torch.cuda.synchronize()
+ready, results = threading.Barrier(8), [None] * 8
+
+def work(n):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        out, adjusted = torch.zeros(1, 1024, dtype=torch.float16, device="cuda"), torch.empty_like(logits)
+        ready.wait()
+        ops.shared_prefix_attention(*args, 1 << 20, 0, pool, pool, out)
+        ops.adjust_logits(logits, adjusted)
+        torch.cuda.current_stream().synchronize()
+        results[n] = out, adjusted
+
+threads = [threading.Thread(target=work, args=(n,)) for n in range(8)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert all(r is not None and torch.equal(r[0], results[0][0]) and torch.equal(r[1], logits) for r in results)
+assert results[0][0].abs().max() > 0
+"""
+
+
+def test_first_calls_of_several_threads_at_once():
+    # in a process of its own, whose kernels' shared-memory limits nobody has raised yet
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS_FROM_SEVERAL_THREADS], timeout=300, cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
