@@ -32,7 +32,7 @@ struct LogitArgs {
 
 // x / repetition for x > 0 without a division (56 us instead of 53.9 for 256 rows of 128256 logits; the product with the
 // reciprocal alone, 52, would be rounded twice). With repetition * scale in [1/2, 1) for a power of two `scale` (in
-// [2^-22, 1) where the repetition is subnormal) the quotient is z / (repetition * scale), z = x * scale. Its product with
+// [2^-23, 1) where the repetition is subnormal) the quotient is z / (repetition * scale), z = x * scale. Its product with
 // the reciprocal is within 1.5 steps, and one residual step (Markstein's: r = z - q b in one rounding, q + r / b) brings
 // it to the nearest float32 but for 2^-22 of a step. Where r could underflow or q overflow the product stands.
 struct Repetition {
