@@ -585,7 +585,7 @@ long long row_tiles(const AttnShape& s, int n_decode, int n_groups, int rows) {
 //    CTA and all of them have a place beside the prefix kernel (two on an SM, where its CTAs of tcgen05 take both and the
 //    others one): none that waits for the shared part keeps another from its keys. Measured: 32 tokens behind 4096 keys,
 //    whose 256 CTAs do not fit beside it, 24.0 us against 20.6 with the third kernel; 48 tokens of 4 KV heads of 32 in two
-//    groups of 777 and 300 keys 9.9 against 11.0.
+//    groups of 777 and 300 keys 9.6 against 11.0.
 //  * `wide`: CTAs of eight warps in the suffix kernel, where each has an SM to itself.
 struct Plan {
   int rows, tiles, parts, slices;
